@@ -4,16 +4,26 @@ ARCH ?= gfx950
 PKG := d-vae_amd
 CSRC := $(PKG)/csrc
 LIB := $(PKG)/lib/libdvae_hip.so
-HDRS := $(wildcard $(CSRC)/*.hpp) include/dvae_hip.h
+LEARN_HDRS := $(CSRC)/layer_norm.hpp $(CSRC)/newton_schulz.hpp
+HDRS := $(filter-out $(LEARN_HDRS),$(wildcard $(CSRC)/*.hpp)) include/dvae_hip.h
+FLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -fno-gpu-rdc -Wall -Wno-unused-function -mllvm -pragma-unroll-threshold=1000000
+# no packed fp32 arithmetic in the kernels (the host pass does not know the feature and says so)
+NO_PK := -Xclang -target-feature -Xclang -packed-fp32-ops
 
 all: $(LIB)
 
-$(LIB): $(CSRC)/dvae_hip.hip $(HDRS)
+$(PKG)/lib/dvae_hip.o: $(CSRC)/dvae_hip.hip $(HDRS)
 	@mkdir -p $(PKG)/lib
-	$(HIPCC) --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -shared -fno-gpu-rdc -Wall -Wno-unused-function -mllvm -pragma-unroll-threshold=1000000 \
-	    -o $@ $(CSRC)/dvae_hip.hip
+	$(HIPCC) $(FLAGS) -c -o $@ $<
+
+$(PKG)/lib/dvae_learn.o: $(CSRC)/dvae_learn.hip $(CSRC)/common.hpp $(LEARN_HDRS) include/dvae_hip.h
+	@mkdir -p $(PKG)/lib
+	$(HIPCC) $(FLAGS) $(NO_PK) -c -o $@ $<
+
+$(LIB): $(PKG)/lib/dvae_hip.o $(PKG)/lib/dvae_learn.o
+	$(HIPCC) --offload-arch=$(ARCH) -fPIC -shared -fno-gpu-rdc -o $@ $^
 
 clean:
-	rm -f $(LIB)
+	rm -f $(LIB) $(PKG)/lib/dvae_hip.o $(PKG)/lib/dvae_learn.o
 
 .PHONY: all clean

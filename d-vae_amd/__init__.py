@@ -8,8 +8,10 @@ from ._lib import BF16, F32
 from .classifier import Evaluator, ResNet18
 from .engine import DVAEConfig, DVAEEngine
 from .model import ResNet18DVAE, ResNetDVAE
-from .optim import FusedAdam
+from .norm import LayerNorm, layer_norm
+from .optim import FusedAdam, FusedMuon, muon_step, newton_schulz
 from .trainer import Trainer, VAE_Trainer, purify_dataset
 
 __all__ = ["_lib", "F32", "BF16", "DVAEConfig", "DVAEEngine", "ResNet18DVAE", "ResNetDVAE", "FusedAdam", "Trainer",
-           "VAE_Trainer", "purify_dataset", "ResNet18", "Evaluator", "classifier", "config", "data", "dist"]
+           "VAE_Trainer", "purify_dataset", "ResNet18", "Evaluator", "classifier", "config", "data", "dist", "LayerNorm",
+           "layer_norm", "FusedMuon", "muon_step", "newton_schulz"]

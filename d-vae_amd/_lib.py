@@ -3,6 +3,7 @@
 The library is built in-tree by ``make`` / ``__graft_entry__.build()``.  There is no fallback: if the
 shared object is missing, every product entry point raises.
 """
+import contextlib
 import ctypes as C
 import os
 
@@ -11,6 +12,7 @@ import torch
 F32, BF16 = 0, 1
 OP_FWD, OP_DGRAD = 0, 1
 NPARTIAL = 1024
+MUON_SPECTRAL, MUON_RMS = 0, 1
 PHILOX_STREAM_16 = 0x80000000     # stream ids with this bit draw eight normals per Philox call from 16-bit uniforms
 SCAL_COUNT = 16
 SCAL = dict(loss=0, loss_rec=1, loss_rec_p=2, loss_p=3, kld=4, gate_kl=5, gate_p=6, grad_norm=7,
@@ -83,6 +85,12 @@ _SIGS = {
     "dvae_poison_u8": (C.c_int, [_P, _P, _P, _P, _P, _L, _I, _I, _P]),
     "dvae_sqnorm_partial": (C.c_int, [_P, _L, _P, _P]),
     "dvae_clip_adam": (C.c_int, [_P, _P, _P, _P, _L, _P, _P, _P, _P]),
+    "dvae_layer_norm_workspace_bytes": (_Z, [_L, _I, _I]),
+    "dvae_layer_norm_fwd": (C.c_int, [_P, _L, _P, _P, _P, _L, _P, _P, _L, _I, _F, _I, _P]),
+    "dvae_layer_norm_bwd": (C.c_int, [_P, _L, _P, _L, _P, _P, _P, _P, _L, _P, _P, _P, _Z, _L, _I, _I, _P]),
+    "dvae_newton_schulz_workspace_bytes": (_Z, [_P, _I]),
+    "dvae_newton_schulz": (C.c_int, [_P, _I, _P, _I, _D, _P, _Z, _I, _P]),
+    "dvae_muon_step": (C.c_int, [_P, _I, _D, _D, _I, _D, _I, _P, _I, _D, _P, _Z, _P]),
 }
 EXPORTS = ["dvae_version", "dvae_last_error"] + list(_SIGS)
 
@@ -127,6 +135,17 @@ def stream():
     if _RAW_STREAM is not None and _CUR_DEVICE is not None:
         return _RAW_STREAM(_CUR_DEVICE())
     return torch.cuda.current_stream().cuda_stream
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def on_device(device):
+    """Context in which the current device is ``device``, a tensor's: launches and allocations of an operator belong there,
+    whatever device its caller has current."""
+    if _CUR_DEVICE is not None and device.index == _CUR_DEVICE():
+        return _NO_GUARD
+    return torch.cuda.device(device)
 
 
 def act_channels(c, dtype=F32):

@@ -15,13 +15,14 @@ import torch
 def _registry():
     from .classifier import ResNet18
     from .model import ResNet18DVAE
-    from .optim import FusedAdam
+    from .optim import FusedAdam, FusedMuon
     return {
         "ResNet18DVAE": ResNet18DVAE,
         "ResNet18": ResNet18,
         "SGD": torch.optim.SGD,
         "Adam": torch.optim.Adam,
         "FusedAdam": FusedAdam,
+        "FusedMuon": FusedMuon,
         "CosineAnnealingLR": torch.optim.lr_scheduler.CosineAnnealingLR,
         "MultiStepLR": torch.optim.lr_scheduler.MultiStepLR,
         "StepLR": torch.optim.lr_scheduler.StepLR,

@@ -1,0 +1,450 @@
+// libdvae_hip.so: entry points of the learning operators that work on tensors of any shape -- layer norm, Newton-Schulz
+// orthogonalisation, the Muon step.  A translation unit of its own: its kernels share nothing with the convolutions'.
+// Host code here only validates, derives launch geometry and launches on the caller's stream.
+#include <limits.h>
+#include <math.h>
+
+#include <vector>
+
+#include "common.hpp"
+#include "layer_norm.hpp"
+#include "newton_schulz.hpp"
+
+using namespace dvae;
+
+namespace {
+
+inline hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
+
+// ---- layer norm -------------------------------------------------------------------------------------------------------
+// How a row is held.  Up to 1024 columns it lives in LPR lanes, NV vectors each; up to 16384 in W waves with at most 16
+// columns a thread; longer rows are read once per pass.
+struct LnShape {
+    int lpr, nv, waves;
+    bool tail;
+};
+inline LnShape ln_shape(int C, int dtype) {
+    const int N = dtype == DVAE_F32 ? 4 : 8;
+    const int vecs = (C + N - 1) / N;
+    LnShape s{0, 1, 0, C % N != 0};
+    if (C <= 1024) {
+        s.lpr = 4;
+        while (s.lpr < vecs && s.lpr < 64) s.lpr <<= 1;
+        while (s.lpr * s.nv < vecs) s.nv <<= 1;
+    } else if (C <= 16384) {
+        s.waves = C <= 4096 ? 4 : C <= 8192 ? 8 : 16;
+        while (s.waves * 64 * s.nv < vecs) s.nv <<= 1;
+    }
+    return s;
+}
+// Workgroups of the backward pass, each of which leaves one slab of column sums: enough to fill the chip several times
+// over, but at least four trips each, so that the slabs stay a small part of the traffic.
+inline int ln_bwd_groups(int64_t rows, int C, int dtype) {
+    const LnShape s = ln_shape(C, dtype);
+    const int64_t rpb = s.lpr ? 256 / s.lpr : 1;
+    int64_t g = cdiv64(rows, rpb * 4);
+    const int64_t cap = s.lpr ? 1024 : s.waves ? 512 : 64;
+    if (g > cap) g = cap;
+    return (int)(g < 1 ? 1 : g);
+}
+
+int ln_check(const char* what, int64_t rows, int C, int dtype) {
+    if (dtype != DVAE_F32 && dtype != DVAE_BF16) DVAE_FAIL(DVAE_EDTYPE, "%s: unknown dtype %d", what, dtype);
+    if (rows < 0 || C <= 0 || C > (1 << 30)) DVAE_FAIL(DVAE_EINVAL, "%s: bad shape %lld x %d", what, (long long)rows, C);
+    return DVAE_OK;
+}
+// an operand: present, element-aligned, rows that do not overlap where they are written
+int ln_operand(const char* what, const char* name, const void* p, int64_t stride, int64_t rows, int C, int dtype, bool written) {
+    const uintptr_t size = dtype == DVAE_F32 ? 4 : 2;
+    if (!p) DVAE_FAIL(DVAE_EINVAL, "%s: %s is null", what, name);
+    if ((uintptr_t)p % size) DVAE_FAIL(DVAE_EINVAL, "%s: %s is not aligned to its elements", what, name);
+    if (stride < 0 || (written && rows > 1 && stride < C))
+        DVAE_FAIL(DVAE_EINVAL, "%s: row stride %lld of %s (%d columns)", what, (long long)stride, name, C);
+    return DVAE_OK;
+}
+
+template <typename T, int LPR, int NV>
+void ln_launch_rows(const LnArgs& a, const LnShape& s, bool bwd, int groups, hipStream_t st) {
+    constexpr int RPB = 256 / LPR, U = NV == 1 ? 4 : NV == 2 ? 2 : 1;
+    if (bwd) {
+        if (s.tail) hipLaunchKernelGGL((ln_bwd_rows_kernel<T, LPR, NV, true>), dim3(groups), dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((ln_bwd_rows_kernel<T, LPR, NV, false>), dim3(groups), dim3(256), 0, st, a);
+        return;
+    }
+    // several rows a lane only where that leaves the chip full: short calls want their rows spread out
+    if (U > 1 && a.rows >= (int64_t)RPB * U * 512) {
+        const int g = (int)(cdiv64(a.rows, RPB * U) < 8192 ? cdiv64(a.rows, RPB * U) : 8192);
+        if (s.tail) hipLaunchKernelGGL((ln_fwd_rows_kernel<T, LPR, NV, U, true>), dim3(g), dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((ln_fwd_rows_kernel<T, LPR, NV, U, false>), dim3(g), dim3(256), 0, st, a);
+    } else {
+        const int g = (int)(cdiv64(a.rows, RPB) < 8192 ? cdiv64(a.rows, RPB) : 8192);
+        if (s.tail) hipLaunchKernelGGL((ln_fwd_rows_kernel<T, LPR, NV, 1, true>), dim3(g), dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((ln_fwd_rows_kernel<T, LPR, NV, 1, false>), dim3(g), dim3(256), 0, st, a);
+    }
+}
+template <typename T, int W, int NV>
+void ln_launch_wide(const LnArgs& a, bool bwd, int groups, hipStream_t st) {
+    if (bwd) hipLaunchKernelGGL((ln_bwd_wide_kernel<T, W, NV>), dim3(groups), dim3(W * 64), 0, st, a);
+    else hipLaunchKernelGGL((ln_fwd_wide_kernel<T, W, NV>), dim3((int)(a.rows < 8192 ? a.rows : 8192)), dim3(W * 64), 0, st, a);
+}
+template <typename T>
+void ln_launch(const LnArgs& a, const LnShape& s, bool bwd, int groups, hipStream_t st) {
+    constexpr bool F = sizeof(T) == 4;                    // bf16 vectors are twice as long: half the count
+    if (s.lpr) {
+        if (s.lpr == 4) ln_launch_rows<T, 4, 1>(a, s, bwd, groups, st);
+        else if (s.lpr == 8) ln_launch_rows<T, 8, 1>(a, s, bwd, groups, st);
+        else if (s.lpr == 16) ln_launch_rows<T, 16, 1>(a, s, bwd, groups, st);
+        else if (s.lpr == 32) ln_launch_rows<T, 32, 1>(a, s, bwd, groups, st);
+        else if (s.nv == 1) ln_launch_rows<T, 64, 1>(a, s, bwd, groups, st);
+        else if (s.nv == 2) ln_launch_rows<T, 64, 2>(a, s, bwd, groups, st);
+        else ln_launch_rows<T, 64, F ? 4 : 2>(a, s, bwd, groups, st);
+    } else if (s.waves == 4) {
+        if (s.nv <= (F ? 2 : 1)) ln_launch_wide<T, 4, F ? 2 : 1>(a, bwd, groups, st);
+        else ln_launch_wide<T, 4, F ? 4 : 2>(a, bwd, groups, st);
+    } else if (s.waves == 8) {
+        ln_launch_wide<T, 8, F ? 4 : 2>(a, bwd, groups, st);
+    } else if (s.waves == 16) {
+        ln_launch_wide<T, 16, F ? 4 : 2>(a, bwd, groups, st);
+    } else if (bwd) {
+        if (a.y) hipLaunchKernelGGL((ln_bwd_long_kernel<T>), dim3((int)(a.rows < 2048 ? a.rows : 2048)), dim3(1024), 0, st, a);
+        if (a.partial) hipLaunchKernelGGL((ln_cols_kernel<T>), dim3((a.C + 255) / 256, groups), dim3(256), 0, st, a);
+    } else {
+        hipLaunchKernelGGL((ln_fwd_long_kernel<T>), dim3((int)(a.rows < 2048 ? a.rows : 2048)), dim3(1024), 0, st, a);
+    }
+}
+
+// ---- Newton-Schulz ----------------------------------------------------------------------------------------------------
+inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+struct NsPlan {
+    std::vector<unsigned> table;      // prefix arrays, then jobs, as they lie on the device
+    int njobs = 0, jp = 0;
+    long total[NS_PHASES] = {0, 0, 0, 0, 0};
+    int gram_ts = 64, sym_ts = 64, apply_ts = 64;
+    bool pieces = false;
+    int kc = 0;
+    size_t norm_off = 0, part_off = 0, bytes = 0;
+    bool matrices = false;
+};
+
+// The largest singular value the iteration can reach from 1, and the largest |a + b s^2 + c s^4| it meets, by the polynomials'
+// own extrema.
+bool ns_coefficients_fit(double a, double b, double c, int steps) {
+    if (!isfinite(a) || !isfinite(b) || !isfinite(c)) return false;
+    auto q = [&](double l) { return a + b * l + c * l * l; };
+    double s = 1.0 + 1e-6;
+    for (int k = 0; k < steps; ++k) {
+        double l[4] = {0.0, s * s, 0.0, 0.0}, most_q = 0.0, most_x = 0.0;
+        int n = 2;
+        if (c != 0.0 && -b / (2 * c) > 0 && -b / (2 * c) < s * s) l[n++] = -b / (2 * c);
+        for (int i = 0; i < n; ++i) most_q = fmax(most_q, fabs(q(l[i])));
+        n = 2;                                            // x q(x^2): a + 3 b l + 5 c l^2 = 0
+        if (c != 0.0) {
+            const double d = 9 * b * b - 20 * a * c;
+            if (d >= 0)
+                for (int g = -1; g <= 1; g += 2) {
+                    const double r = (-3 * b + g * sqrt(d)) / (10 * c);
+                    if (r > 0 && r < s * s) l[n++] = r;
+                }
+        } else if (b != 0.0 && -a / (3 * b) > 0 && -a / (3 * b) < s * s) {
+            l[n++] = -a / (3 * b);
+        }
+        for (int i = 0; i < n; ++i) most_x = fmax(most_x, sqrt(l[i]) * fabs(q(l[i])));
+        if (!(most_q <= 7.001)) return false;                // a hair over, so that the bounds themselves pass
+        s = most_x * (1.0 + 1e-4);
+        if (!(s <= 2.001)) return false;
+        if (s == 0.0) return true;
+        if (s < 1e-30) s = 1e-30;
+    }
+    return true;
+}
+
+int ns_check(const char* what, const dvae_matrix* mats, int count, int dtype, bool muon) {
+    if (count < 0 || (count > 0 && !mats)) DVAE_FAIL(DVAE_EINVAL, "%s: null list", what);
+    if (count > 65536) DVAE_FAIL(DVAE_EINVAL, "%s: %d matrices (65536 at most)", what, count);
+    if (dtype != DVAE_F32 && dtype != DVAE_BF16) DVAE_FAIL(DVAE_EDTYPE, "%s: unknown dtype %d", what, dtype);
+    for (int i = 0; i < count; ++i) {
+        const dvae_matrix& m = mats[i];
+        const uintptr_t size = dtype == DVAE_F32 ? 4 : 2;
+        if (m.rows <= 0 || m.cols <= 0 || m.rows > (1 << 30) || m.cols > (1 << 30) || m.rows * m.cols >= (1LL << 31))
+            DVAE_FAIL(DVAE_EINVAL, "%s: matrix %d is %lld x %lld", what, i, (long long)m.rows, (long long)m.cols);
+        if (!m.x || !m.out || (muon && !m.momentum)) DVAE_FAIL(DVAE_EINVAL, "%s: matrix %d has a null pointer", what, i);
+        if (((uintptr_t)m.x | (uintptr_t)m.out) % size || (muon && (uintptr_t)m.momentum % 4))
+            DVAE_FAIL(DVAE_EINVAL, "%s: matrix %d is not aligned to its elements", what, i);
+        if (muon ? m.x_stride != m.cols || m.out_stride != m.cols : m.x_stride < 0 || (m.rows > 1 && m.out_stride < m.cols))
+            DVAE_FAIL(DVAE_EINVAL, "%s: matrix %d has row strides %lld, %lld", what, i, (long long)m.x_stride, (long long)m.out_stride);
+    }
+    return DVAE_OK;
+}
+
+inline long ns_triangles(int P, int ts) {
+    const long t = (P + ts - 1) / ts;
+    return t * (t + 1) / 2;
+}
+
+int ns_plan(const char* what, const dvae_matrix* mats, int count, int scale_rule, NsPlan& p) {
+    p.njobs = count;
+    p.jp = (count + 1 + 63) / 64 * 64;
+    std::vector<NsJob> jobs((size_t)count);
+    std::vector<int> first((size_t)NS_PHASES * p.jp, INT_MAX);
+    // Tiles of 128 read half as much LDS per product as tiles of 64, and want enough of them: the larger tile is taken
+    // where its tiles alone give every CU one.
+    long big_apply = 0, big_sym = 0, sym64 = 0, lines64 = 0;
+    for (int i = 0; i < count; ++i) {
+        const dvae_matrix& m = mats[i];
+        if (m.vector) continue;
+        const long P = ns_pad((int)(m.rows < m.cols ? m.rows : m.cols)), Q = ns_pad((int)(m.rows < m.cols ? m.cols : m.rows));
+        big_apply += (P + 127) / 128 * ((Q + 127) / 128);
+        big_sym += ns_triangles((int)P, 128);
+        sym64 += ns_triangles((int)P, 64);
+        lines64 += ns_triangles((int)P, 64) * (Q / 32);
+        p.matrices = true;
+    }
+    p.apply_ts = big_apply >= 256 ? 128 : 64;
+    p.sym_ts = big_sym >= 256 ? 128 : 64;
+    p.gram_ts = p.sym_ts;
+    // The Gram phase has few tiles and a long contraction: below 512 workgroups it is cut into pieces of equal length.
+    if (p.gram_ts == 64 && sym64 < 512) {
+        p.kc = (int)((lines64 + 511) / 512);
+        if (p.kc < 4) p.kc = 4;
+    }
+    long off = 0, part = 0;
+    for (int i = 0; i < count; ++i) {
+        const dvae_matrix& m = mats[i];
+        NsJob& j = jobs[i];
+        j.x = m.x; j.out = m.out; j.mom = m.momentum;
+        j.xs = m.x_stride; j.os = m.out_stride;
+        j.m = (int)m.rows; j.n = (int)m.cols;
+        j.vec = m.vector ? 1 : 0;
+        const long chunks = ((long)j.m * j.n + NS_CHUNK - 1) / NS_CHUNK;
+        j.nchunk = (int)(chunks < 1024 ? chunks : 1024);
+        j.part = (int)part;
+        const double r = (double)j.m, c = (double)j.n;
+        j.scale = (float)(scale_rule == DVAE_MUON_RMS ? 0.2 * sqrt(fmax(r, c)) : sqrt(fmax(1.0, r / c)));
+        for (int f = 0; f < NS_PHASES; ++f) {
+            if (p.total[f] > INT_MAX / 2) DVAE_FAIL(DVAE_EINVAL, "%s: too much work for one call", what);
+            first[(size_t)f * p.jp + i] = (int)p.total[f];
+        }
+        p.total[NS_NORM] += j.nchunk;
+        j.off = off;
+        if (j.vec) continue;
+        part += j.nchunk;
+        const int P = ns_pad(j.m < j.n ? j.m : j.n), Q = ns_pad(j.m < j.n ? j.n : j.m);
+        off += ns_job_bytes(j.m, j.n);
+        p.total[NS_SPLIT] += (long)(P / 64) * (Q / 64);
+        const long pieces = p.kc ? (Q / 32 + p.kc - 1) / p.kc : 1;
+        if (pieces > 1) p.pieces = true;
+        p.total[NS_GRAM] += ns_triangles(P, p.gram_ts) * pieces;
+        p.total[NS_SYM] += ns_triangles(P, p.sym_ts);
+        p.total[NS_APPLY] += (long)((P + p.apply_ts - 1) / p.apply_ts) * ((Q + p.apply_ts - 1) / p.apply_ts);
+    }
+    for (int f = 0; f < NS_PHASES; ++f)
+        if (p.total[f] > INT_MAX / 2) DVAE_FAIL(DVAE_EINVAL, "%s: too much work for one call", what);
+    // jobs without tiles in a phase share their first with the next one that has some; those after the last such are beyond it
+    const size_t words = first.size() + jobs.size() * sizeof(NsJob) / 4;
+    p.table.resize(words);
+    memcpy(p.table.data(), first.data(), first.size() * 4);
+    if (count) memcpy(p.table.data() + first.size(), jobs.data(), jobs.size() * sizeof(NsJob));
+    p.norm_off = align256(words * 4);
+    p.part_off = p.norm_off + align256((size_t)part * sizeof(double));
+    const size_t planes = p.part_off + (p.pieces ? align256((size_t)p.total[NS_GRAM] * 64 * 64 * 4) : 0);
+    NsJob* t = reinterpret_cast<NsJob*>(p.table.data() + first.size());
+    for (int i = 0; i < count; ++i) t[i].off += (long)planes;
+    p.bytes = planes + (size_t)off;
+    return DVAE_OK;
+}
+
+template <typename T, bool MUON>
+int ns_run(const char* what, const NsPlan& p, NsArgs g, int steps, hipStream_t st) {
+    // the table, as many kernel arguments at a time as fit
+    NsBlob blob;
+    for (size_t at = 0; at < p.table.size(); at += NsBlob::WORDS) {
+        const size_t n = p.table.size() - at < (size_t)NsBlob::WORDS ? p.table.size() - at : (size_t)NsBlob::WORDS;
+        memcpy(blob.w, p.table.data() + at, n * 4);
+        hipLaunchKernelGGL(ns_table_kernel, dim3(1), dim3(256), 0, st, blob, (unsigned*)g.ws + at, (int)n);
+        DVAE_CHECK_LAUNCH(what);
+    }
+    g.first = (const int*)g.ws;
+    g.jobs = (const NsJob*)(g.ws + (size_t)NS_PHASES * p.jp * 4);
+    g.norm = (double*)(g.ws + p.norm_off);
+    g.part = (float*)(g.ws + p.part_off);
+    g.njobs = p.njobs;
+    g.jp = p.jp;
+    g.kc = p.kc;
+    g.turn = 0;
+#define NS_LAUNCH(kernel, phase)                                                                     \
+    do {                                                                                             \
+        g.total = (int)p.total[phase];                                                               \
+        hipLaunchKernelGGL((kernel), dim3((unsigned)p.total[phase]), dim3(256), 0, st, g);           \
+        DVAE_CHECK_LAUNCH(what);                                                                     \
+    } while (0)
+    NS_LAUNCH((ns_norm_kernel<T, MUON>), NS_NORM);
+    if (!p.matrices) return DVAE_OK;
+    NS_LAUNCH((ns_split_kernel<T, MUON>), NS_SPLIT);
+    for (int k = 0; k < steps; ++k) {
+        if (p.pieces) {
+            NS_LAUNCH((ns_gram_kernel<64, true>), NS_GRAM);
+            NS_LAUNCH(ns_gram_sum_kernel<64>, NS_SYM);
+        } else if (p.gram_ts == 128) {
+            NS_LAUNCH((ns_gram_kernel<128, false>), NS_GRAM);
+        } else {
+            NS_LAUNCH((ns_gram_kernel<64, false>), NS_GRAM);
+        }
+        if (p.sym_ts == 128) NS_LAUNCH(ns_square_kernel<128>, NS_SYM);
+        else NS_LAUNCH(ns_square_kernel<64>, NS_SYM);
+        if (k + 1 < steps) {
+            if (p.apply_ts == 128) NS_LAUNCH(ns_apply_kernel<128>, NS_APPLY);
+            else NS_LAUNCH(ns_apply_kernel<64>, NS_APPLY);
+            g.turn ^= 1;
+        } else if (p.apply_ts == 128) {
+            NS_LAUNCH((ns_last_kernel<128, T, MUON>), NS_APPLY);
+        } else {
+            NS_LAUNCH((ns_last_kernel<64, T, MUON>), NS_APPLY);
+        }
+    }
+#undef NS_LAUNCH
+    return DVAE_OK;
+}
+
+int ns_iteration_check(const char* what, const double* coefficients, int steps, double eps) {
+    if (!coefficients) DVAE_FAIL(DVAE_EINVAL, "%s: null coefficients", what);
+    if (steps < 1 || steps > 100) DVAE_FAIL(DVAE_EINVAL, "%s: %d steps (1 to 100)", what, steps);
+    if (!(eps >= 0.0) || !isfinite(eps)) DVAE_FAIL(DVAE_EINVAL, "%s: eps %g", what, eps);
+    if (!ns_coefficients_fit(coefficients[0], coefficients[1], coefficients[2], steps))
+        DVAE_FAIL(DVAE_EINVAL, "%s: coefficients (%g, %g, %g) leave the range this iteration is computed in: from singular "
+                  "values up to 1 every step has to stay at 2 or below, with |a + b s^2 + c s^4| at 7 or below", what,
+                  coefficients[0], coefficients[1], coefficients[2]);
+    return DVAE_OK;
+}
+int ns_workspace_check(const char* what, const void* ws, size_t have, size_t need) {
+    if (!ws || (uintptr_t)ws & 255) DVAE_FAIL(DVAE_EINVAL, "%s: the workspace must be 256-byte aligned", what);
+    if (have < need) DVAE_FAIL(DVAE_EWORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, have, need);
+    return DVAE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t dvae_layer_norm_workspace_bytes(int64_t rows, int C, int dtype) {
+    if (rows < 0 || C <= 0 || (dtype != DVAE_F32 && dtype != DVAE_BF16)) return 0;
+    return (size_t)ln_bwd_groups(rows, C, dtype) * 2 * C * sizeof(float);
+}
+
+int dvae_layer_norm_fwd(const void* x, int64_t x_stride, const float* gamma, const float* beta, void* y, int64_t y_stride,
+                        float* save_mean, float* save_invstd, int64_t rows, int C, float eps, int dtype, void* st) {
+    int rc = ln_check("layer_norm_fwd", rows, C, dtype);
+    if (rc || rows == 0) return rc;
+    if ((rc = ln_operand("layer_norm_fwd", "x", x, x_stride, rows, C, dtype, false))) return rc;
+    if ((rc = ln_operand("layer_norm_fwd", "y", y, y_stride, rows, C, dtype, true))) return rc;
+    if (!save_mean != !save_invstd) DVAE_FAIL(DVAE_EINVAL, "layer_norm_fwd: save_mean and save_invstd go together");
+    if (!(eps >= 0.f)) DVAE_FAIL(DVAE_EINVAL, "layer_norm_fwd: eps %g", eps);
+    LnArgs a{};
+    a.x = x; a.xs = x_stride; a.y = y; a.ys = y_stride; a.gamma = gamma; a.beta = beta; a.mean = save_mean; a.invstd = save_invstd;
+    a.rows = rows; a.C = C; a.eps = eps;
+    const LnShape s = ln_shape(C, dtype);
+    if (dtype == DVAE_F32) ln_launch<float>(a, s, false, 0, S(st));
+    else ln_launch<bf16>(a, s, false, 0, S(st));
+    DVAE_CHECK_LAUNCH("layer_norm_fwd");
+    return DVAE_OK;
+}
+
+int dvae_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const float* gamma,
+                        const float* save_mean, const float* save_invstd, void* dx, int64_t dx_stride, float* dgamma,
+                        float* dbeta, void* workspace, size_t workspace_bytes, int64_t rows, int C, int dtype, void* st) {
+    int rc = ln_check("layer_norm_bwd", rows, C, dtype);
+    if (rc) return rc;
+    const bool sums = dgamma || dbeta;
+    if (!dx && !sums) return DVAE_OK;
+    const int groups = ln_bwd_groups(rows, C, dtype);
+    if (sums && rows) {
+        if (!workspace || (uintptr_t)workspace & 15) DVAE_FAIL(DVAE_EINVAL, "layer_norm_bwd: the workspace must be 16-byte aligned");
+        if (workspace_bytes < dvae_layer_norm_workspace_bytes(rows, C, dtype))
+            DVAE_FAIL(DVAE_EWORKSPACE, "layer_norm_bwd: workspace of %zu bytes, %zu needed", workspace_bytes,
+                      dvae_layer_norm_workspace_bytes(rows, C, dtype));
+    }
+    if (rows) {
+        if ((rc = ln_operand("layer_norm_bwd", "dy", dy, dy_stride, rows, C, dtype, false))) return rc;
+        if ((rc = ln_operand("layer_norm_bwd", "x", x, x_stride, rows, C, dtype, false))) return rc;
+        if (dx && (rc = ln_operand("layer_norm_bwd", "dx", dx, dx_stride, rows, C, dtype, true))) return rc;
+        if (!save_mean || !save_invstd) DVAE_FAIL(DVAE_EINVAL, "layer_norm_bwd: the forward pass's statistics are missing");
+        LnArgs a{};
+        a.x = x; a.xs = x_stride; a.dy = dy; a.ds = dy_stride; a.y = dx; a.ys = dx_stride; a.gamma = gamma;
+        a.mean = const_cast<float*>(save_mean); a.invstd = const_cast<float*>(save_invstd);
+        a.partial = sums ? (float*)workspace : nullptr;
+        a.rows = rows; a.C = C;
+        const LnShape s = ln_shape(C, dtype);
+        if (dtype == DVAE_F32) ln_launch<float>(a, s, true, groups, S(st));
+        else ln_launch<bf16>(a, s, true, groups, S(st));
+        DVAE_CHECK_LAUNCH("layer_norm_bwd");
+    }
+    if (sums) {
+        hipLaunchKernelGGL(ln_reduce_kernel, dim3((unsigned)cdiv64(2LL * C, 64)), dim3(256), 0, S(st), (const float*)workspace,
+                           rows ? groups : 0, C, dgamma, dbeta);
+        DVAE_CHECK_LAUNCH("layer_norm_bwd");
+    }
+    return DVAE_OK;
+}
+
+size_t dvae_newton_schulz_workspace_bytes(const dvae_matrix* mats, int count) {
+    try {
+        if (count < 0 || (count > 0 && !mats) || count > 65536) return 0;
+        for (int i = 0; i < count; ++i)
+            if (mats[i].rows <= 0 || mats[i].cols <= 0 || mats[i].rows > (1 << 30) || mats[i].cols > (1 << 30) ||
+                mats[i].rows * mats[i].cols >= (1LL << 31)) return 0;
+        NsPlan p;
+        return ns_plan("newton_schulz", mats, count, DVAE_MUON_SPECTRAL, p) ? 0 : p.bytes;
+    } catch (...) {
+        return 0;
+    }
+}
+
+int dvae_newton_schulz(const dvae_matrix* mats, int count, const double* coefficients, int steps, double eps, void* workspace,
+                       size_t workspace_bytes, int dtype, void* st) {
+    try {
+        int rc = ns_check("newton_schulz", mats, count, dtype, false);
+        if (rc) return rc;
+        if ((rc = ns_iteration_check("newton_schulz", coefficients, steps, eps))) return rc;
+        for (int i = 0; i < count; ++i)
+            if (mats[i].vector) DVAE_FAIL(DVAE_EINVAL, "newton_schulz: matrix %d is marked as a vector", i);
+        if (count == 0) return DVAE_OK;
+        NsPlan p;
+        if ((rc = ns_plan("newton_schulz", mats, count, DVAE_MUON_SPECTRAL, p))) return rc;
+        if ((rc = ns_workspace_check("newton_schulz", workspace, workspace_bytes, p.bytes))) return rc;
+        NsArgs g{};
+        g.ws = (char*)workspace;
+        g.a = (float)coefficients[0]; g.b = (float)coefficients[1]; g.c = (float)coefficients[2];
+        g.eps = eps;
+        return dtype == DVAE_F32 ? ns_run<float, false>("newton_schulz", p, g, steps, S(st))
+                                 : ns_run<bf16, false>("newton_schulz", p, g, steps, S(st));
+    } catch (...) {
+        DVAE_FAIL(DVAE_EINVAL, "newton_schulz: out of host memory");
+    }
+}
+
+int dvae_muon_step(const dvae_matrix* mats, int count, double lr, double momentum, int nesterov, double weight_decay, int scale_rule,
+                   const double* coefficients, int steps, double eps, void* workspace, size_t workspace_bytes, void* st) {
+    try {
+        int rc = ns_check("muon_step", mats, count, DVAE_F32, true);
+        if (rc) return rc;
+        if ((rc = ns_iteration_check("muon_step", coefficients, steps, eps))) return rc;
+        if (scale_rule != DVAE_MUON_SPECTRAL && scale_rule != DVAE_MUON_RMS) DVAE_FAIL(DVAE_EINVAL, "muon_step: scale rule %d", scale_rule);
+        if (!(momentum >= 0.0 && momentum < 1.0) || !(lr >= 0.0) || !(weight_decay >= 0.0) || !isfinite(lr * weight_decay))
+            DVAE_FAIL(DVAE_EINVAL, "muon_step: lr %g, momentum %g, weight decay %g", lr, momentum, weight_decay);
+        if (count == 0) return DVAE_OK;
+        NsPlan p;
+        if ((rc = ns_plan("muon_step", mats, count, scale_rule, p))) return rc;
+        if ((rc = ns_workspace_check("muon_step", workspace, workspace_bytes, p.bytes))) return rc;
+        NsArgs g{};
+        g.ws = (char*)workspace;
+        g.a = (float)coefficients[0]; g.b = (float)coefficients[1]; g.c = (float)coefficients[2];
+        g.eps = eps;
+        g.mu = (float)momentum; g.nu = (float)(1.0 - momentum); g.nesterov = nesterov; g.lr = (float)lr;
+        g.decay = (float)(1.0 - lr * weight_decay);
+        return ns_run<float, true>("muon_step", p, g, steps, S(st));
+    } catch (...) {
+        DVAE_FAIL(DVAE_EINVAL, "muon_step: out of host memory");
+    }
+}
+
+}  // extern "C"

@@ -6,8 +6,167 @@ weight_decay 0: configs/cifar10/resnet18DVAE.yaml:21-23) with two launches of li
 ``torch.optim.Optimizer`` so the reference's ``config_s.scheduler(optimizer)`` (CosineAnnealingLR) and
 ``optimizer.param_groups[0]['lr']`` keep working.  Parameters off the hot path never receive a
 gradient in the D-VAE stage (as in the reference, where Adam skips ``grad is None``) and are not touched.
+
+Beside it, for any float32 parameters (the D-VAE's through autograd, the classifier's): ``FusedMuon``, whose step moves a
+matrix by its momentum's nearest orthogonal matrix instead of the momentum itself, with ``muon_step`` and ``newton_schulz``,
+the operators under it.  They have no counterpart in the reference.
 """
+from array import array
+import math
+
 import torch
+
+from . import _lib as L
+
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+_SCALES = {"spectral": L.MUON_SPECTRAL, "rms": L.MUON_RMS}
+
+
+def _workspace(table, count, device):
+    n = L.lib().dvae_newton_schulz_workspace_bytes(table, count)
+    return torch.empty(n, dtype=torch.uint8, device=device), n
+
+
+def newton_schulz(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
+    """Orthogonalises matrices: X / (|X|_F + eps), then ``steps`` times X <- a X + (b A + c A^2) X with A = X X^T and
+    (a, b, c) = ``coefficients``, which drives every singular value towards 1 and leaves the singular vectors.
+
+    ``x``: a float32 or bfloat16 device tensor of shape [..., m, n], or a list of them of one type (any shapes: the whole list
+    is one batch of launches).  Returns the same, in x's type.  The products have float32 accuracy for either type.  The
+    result is not differentiable."""
+    many = isinstance(x, (list, tuple))
+    xs = list(x) if many else [x]
+    outs, table, keep = [], array("q"), []
+    for i, t in enumerate(xs):
+        if not t.is_cuda:
+            raise RuntimeError("newton_schulz runs on libdvae_hip: it takes device tensors")
+        if t.dtype not in (torch.float32, torch.bfloat16) or t.dtype != xs[0].dtype or t.device != xs[0].device:
+            raise RuntimeError(f"newton_schulz: tensor {i} is {t.dtype} on {t.device}; all have to be float32 or all bfloat16, "
+                               "on one device")
+        if t.dim() < 2:
+            raise RuntimeError(f"newton_schulz: tensor {i} of shape {tuple(t.shape)} is no matrix")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("newton_schulz is not differentiable: pass a detached tensor or call it under torch.no_grad()")
+        m, n = t.shape[-2:]
+        if t.numel() == 0:
+            outs.append(torch.empty(t.shape, dtype=t.dtype, device=t.device))
+            continue
+        flat = t.detach()
+        flip = not (flat.stride(-1) == 1 or n == 1) and (flat.stride(-2) == 1 or m == 1)
+        if flip:                                     # stored by columns: the transpose is what lies in memory
+            flat, m, n = flat.mT, n, m
+        flat = flat.reshape(-1, m, n)
+        if not (flat.stride(2) == 1 or n == 1):
+            flat = flat.contiguous()
+        keep.append(flat)
+        out = torch.empty(t.shape[:-2] + (m, n), dtype=t.dtype, device=t.device)
+        outs.append(out.mT if flip else out)
+        size, src, dst = t.element_size(), flat.data_ptr(), out.data_ptr()
+        step = flat.stride(0) * size
+        stride = flat.stride(1)
+        for b in range(flat.shape[0]):
+            table.extend((src + b * step, dst + b * m * n * size, 0, m, n, stride, n, 0))
+    count = len(table) // 8
+    if count:
+        device = xs[0].device
+        with L.on_device(device):
+            at = table.buffer_info()[0]
+            ws, size = _workspace(at, count, device)
+            coef = array("d", coefficients)
+            if len(coef) != 3:
+                raise RuntimeError(f"newton_schulz: three coefficients, got {len(coef)}")
+            L.check(L.lib().dvae_newton_schulz(at, count, coef.buffer_info()[0], int(steps), float(eps), ws.data_ptr(), size,
+                                               L.F32 if xs[0].dtype == torch.float32 else L.BF16, L.stream()))
+    return outs if many else outs[0]
+
+
+@torch.no_grad()
+def muon_step(params, grads, momenta, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5,
+              coefficients=COEFFICIENTS, eps=1e-7, scale="spectral"):
+    """One Muon step, in place, over lists of contiguous float32 device tensors that share no memory:
+
+        m <- momentum m + (1 - momentum) g;   u = (1 - momentum) g + momentum m  (nesterov; else m)
+        p <- p (1 - lr weight_decay) - lr s newton_schulz(u)
+
+    with every parameter of two or more dimensions taken as the matrix [shape[0], rest] and s = sqrt(max(1, rows / cols))
+    (``scale="spectral"``) or 0.2 sqrt(max(rows, cols)) (``"rms"``: steps as long as Adam's).  Parameters of fewer dimensions
+    (gains, biases) move by lr u.  All parameters go through the same dozen and a half launches."""
+    if not len(params) == len(grads) == len(momenta):
+        raise RuntimeError(f"muon_step: {len(params)} parameters, {len(grads)} gradients, {len(momenta)} momenta")
+    if scale not in _SCALES:
+        raise RuntimeError(f"muon_step: scale {scale!r} ({sorted(_SCALES)})")
+    table, written, read = array("q"), set(), set()
+    device = params[0].device if params else None
+    for i, (p, g, m) in enumerate(zip(params, grads, momenta)):
+        shape = p.shape
+        for what, t in (("parameter", p), ("gradient", g), ("momentum", m)):
+            if t.dtype != torch.float32 or not t.is_cuda or t.device != device or t.shape != shape or not t.is_contiguous():
+                raise RuntimeError(f"muon_step: {what} {i} must be a contiguous float32 tensor of shape {tuple(shape)} on one "
+                                   f"device, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        n = p.numel()
+        if n == 0:
+            continue
+        pp, gp, mp = p.data_ptr(), g.data_ptr(), m.data_ptr()
+        written.add(pp)
+        written.add(mp)
+        read.add(gp)
+        if len(shape) < 2:
+            table.extend((gp, pp, mp, 1, n, n, n, 1))
+        else:
+            cols = n // shape[0]
+            table.extend((gp, pp, mp, shape[0], cols, cols, cols, 0))
+    count = len(table) // 8
+    if len(written) != 2 * count or not written.isdisjoint(read):
+        raise RuntimeError("muon_step: a parameter or momentum is listed twice")
+    if not count:
+        return
+    with L.on_device(device):
+        at = table.buffer_info()[0]
+        ws, size = _workspace(at, count, device)
+        coef = array("d", coefficients)
+        if len(coef) != 3:
+            raise RuntimeError(f"muon_step: three coefficients, got {len(coef)}")
+        L.check(L.lib().dvae_muon_step(at, count, lr, momentum, int(nesterov), weight_decay, _SCALES[scale],
+                                       coef.buffer_info()[0], int(steps), float(eps), ws.data_ptr(), size, L.stream()))
+    torch.autograd.graph.increment_version([*params, *momenta])     # packed weights and saved tensors notice the step
+
+
+class FusedMuon(torch.optim.Optimizer):
+    """Muon over ``muon_step``: a torch optimiser (schedulers, param groups, ``state_dict``) for float32 device parameters.
+    Parameters without a gradient are skipped.  Groups may differ in any option; each group is one batch of launches.  A step
+    captured into a graph keeps the options it was captured with."""
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=COEFFICIENTS,
+                 eps=1e-7, scale="spectral"):
+        if not (lr >= 0.0 and math.isfinite(lr)) or not 0.0 <= momentum < 1.0 or not weight_decay >= 0.0:
+            raise ValueError(f"FusedMuon: lr {lr}, momentum {momentum}, weight_decay {weight_decay}")
+        if scale not in _SCALES:
+            raise ValueError(f"FusedMuon: scale {scale!r} ({sorted(_SCALES)})")
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
+                                      coefficients=tuple(coefficients), eps=eps, scale=scale))
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            params = [p for p in group["params"] if p.grad is not None]
+            if not params:
+                continue
+            momenta = []
+            for p in params:
+                state = self.state[p]
+                if "momentum_buffer" not in state:
+                    state["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
+                momenta.append(state["momentum_buffer"])
+            muon_step(params, [p.grad.contiguous() for p in params], momenta,
+                      **{k: v for k, v in group.items() if k in self.defaults and k in _STEP_OPTIONS})
+        return loss
+
+
+_STEP_OPTIONS = ("lr", "momentum", "nesterov", "weight_decay", "steps", "coefficients", "eps", "scale")
 
 
 class FusedAdam(torch.optim.Optimizer):

@@ -297,6 +297,48 @@ int dvae_sqnorm_partial(const float* g, int64_t n, float* partial /* [DVAE_NPART
 int dvae_clip_adam(float* p, const float* g, float* m, float* v, int64_t n, float* hyper,
                    const float* partial, float* scal, void* stream);
 
+/* ---- layer norm over the last dimension (nn.LayerNorm; beside the batch and instance norms above) ----------------------
+ * x, y, dy, dx: `rows` rows of C elements of `dtype`, each tensor with a row stride of its own in elements (an activation
+ * map whose channels are padded passes its padded width; columns past C are neither read nor written; a stride of 0 repeats
+ * one input row).  Pointers need the alignment of one element only.  gamma, beta and their gradients are fp32 [C], each
+ * NULL if absent.  save_mean / save_invstd (fp32 [rows], both or neither) are what the backward pass reads; inference
+ * passes NULL.  dx, dgamma and dbeta may each be NULL.  The workspace (16-byte aligned) is needed only for dgamma / dbeta.
+ * rows == 0 is allowed: the gradients of gamma and beta are then zero.  Bitwise reproducible; a row's results do not depend
+ * on the other rows. */
+size_t dvae_layer_norm_workspace_bytes(int64_t rows, int C, int dtype);
+int dvae_layer_norm_fwd(const void* x, int64_t x_stride, const float* gamma, const float* beta, void* y, int64_t y_stride,
+                        float* save_mean, float* save_invstd, int64_t rows, int C, float eps, int dtype, void* stream);
+int dvae_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const float* gamma,
+                        const float* save_mean, const float* save_invstd, void* dx, int64_t dx_stride, float* dgamma,
+                        float* dbeta, void* workspace, size_t workspace_bytes, int64_t rows, int C, int dtype, void* stream);
+
+/* ---- Newton-Schulz orthogonalisation and the Muon step (an optimiser beside dvae_clip_adam) ------------------------------
+ * One call takes a list of matrices of any shapes (rows * cols < 2^31 each); the list is host memory and is read before the
+ * call returns, whatever it points to is device memory.  Every matrix is divided by |X|_F + eps and goes `steps` times through
+ *     A = X X^T,  X <- a X + (b A + c A^2) X        (coefficients = {a, b, c}; with rows > cols, as its transpose),
+ * in products of fp32 accuracy whatever `dtype`, the type of x and out, is.  The coefficients have to keep the iteration
+ * within singular values of 2 and |a + b s^2 + c s^4| within 7 (those in use do), else DVAE_EINVAL.  A matrix with a
+ * non-finite element gives NaNs, a zero matrix zeros.  The workspace is 256-byte aligned. */
+typedef struct dvae_matrix {
+    const void* x;            /* the matrix; dvae_muon_step: its gradient, fp32 */
+    void* out;                /* the result; dvae_muon_step: the parameter, fp32, stepped in place */
+    float* momentum;          /* dvae_muon_step: stepped in place; else NULL */
+    int64_t rows, cols;
+    int64_t x_stride, out_stride;   /* between rows, in elements; dvae_muon_step: both = cols */
+    int64_t vector;           /* dvae_muon_step: 1 = takes the momentum step without orthogonalisation (gains, biases) */
+} dvae_matrix;
+size_t dvae_newton_schulz_workspace_bytes(const dvae_matrix* list, int count);   /* of dvae_muon_step too */
+int dvae_newton_schulz(const dvae_matrix* list, int count, const double* coefficients, int steps, double eps, void* workspace,
+                       size_t workspace_bytes, int dtype, void* stream);
+/* m <- momentum m + (1 - momentum) g;  u = (1 - momentum) g + momentum m  (nesterov; else u = m)
+ * p <- p (1 - lr weight_decay) - lr s O, with O the orthogonalised u and s = sqrt(max(1, rows / cols)) (DVAE_MUON_SPECTRAL)
+ * or 0.2 sqrt(max(rows, cols)) (DVAE_MUON_RMS); vectors: O = u, s = 1.  No two entries may share memory. */
+#define DVAE_MUON_SPECTRAL 0
+#define DVAE_MUON_RMS 1
+int dvae_muon_step(const dvae_matrix* list, int count, double lr, double momentum, int nesterov, double weight_decay,
+                   int scale_rule, const double* coefficients, int steps, double eps, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif
