@@ -17,8 +17,9 @@ namespace {
 inline hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
 // ---- layer norm -------------------------------------------------------------------------------------------------------
-// How a row is held.  Up to 1024 columns it lives in LPR lanes, NV vectors each; up to 16384 in W waves with at most 16
-// columns a thread; longer rows are read once per pass.
+// How a row is held.  Up to 512 columns it lives in LPR lanes of at most 8 columns; up to 8192 in W waves, 8 columns a thread
+// again (16 take twice the registers of the backward pass and half its occupancy: 3.0 instead of 4.4 TB/s at 4096 bf16
+// columns); up to 16384 in 16 waves with 16; longer rows are read once per pass.
 struct LnShape {
     int lpr, nv, waves;
     bool tail;
@@ -27,26 +28,30 @@ inline LnShape ln_shape(int C, int dtype) {
     const int N = dtype == DVAE_F32 ? 4 : 8;
     const int vecs = (C + N - 1) / N;
     LnShape s{0, 1, 0, C % N != 0};
-    if (C <= 1024) {
+    if (C <= 512) {
         s.lpr = 4;
         while (s.lpr < vecs && s.lpr < 64) s.lpr <<= 1;
         while (s.lpr * s.nv < vecs) s.nv <<= 1;
     } else if (C <= 16384) {
-        s.waves = C <= 4096 ? 4 : C <= 8192 ? 8 : 16;
-        while (s.waves * 64 * s.nv < vecs) s.nv <<= 1;
+        s.waves = 2;
+        while (s.waves < 16 && s.waves * 512 < C) s.waves <<= 1;
+        s.nv = (C <= 8192 ? 8 : 16) / N;
     }
     return s;
 }
-// Workgroups of the backward pass, each of which leaves one slab of column sums: enough to fill the chip several times
-// over, but at least four trips each, so that the slabs stay a small part of the traffic.
+// Workgroups of the backward pass, each of which leaves one slab of column sums: enough to fill the chip, but at least four
+// trips each, so that the slabs stay a small part of the traffic.
 inline int ln_bwd_groups(int64_t rows, int C, int dtype) {
     const LnShape s = ln_shape(C, dtype);
     const int64_t rpb = s.lpr ? 256 / s.lpr : 1;
     int64_t g = cdiv64(rows, rpb * 4);
-    const int64_t cap = s.lpr ? 1024 : s.waves ? 512 : 64;
+    if (g > 256) g = cdiv64(rows, rpb * 8) > 256 ? cdiv64(rows, rpb * 8) : 256;      // eight trips once every CU has one
+    const int64_t cap = s.lpr || s.waves <= 4 ? 1024 : s.waves ? 4096 / s.waves : 64;
     if (g > cap) g = cap;
     return (int)(g < 1 ? 1 : g);
 }
+// Forward: eight workgroups of four waves a CU, which then walk their rows with gamma / beta in registers.
+constexpr int LN_GRID = 2048;
 
 int ln_check(const char* what, int64_t rows, int C, int dtype) {
     if (dtype != DVAE_F32 && dtype != DVAE_BF16) DVAE_FAIL(DVAE_EDTYPE, "%s: unknown dtype %d", what, dtype);
@@ -65,7 +70,7 @@ int ln_operand(const char* what, const char* name, const void* p, int64_t stride
 
 template <typename T, int LPR, int NV>
 void ln_launch_rows(const LnArgs& a, const LnShape& s, bool bwd, int groups, hipStream_t st) {
-    constexpr int RPB = 256 / LPR, U = NV == 1 ? 4 : NV == 2 ? 2 : 1;
+    constexpr int RPB = 256 / LPR, U = NV == 1 ? 4 : 2;
     if (bwd) {
         if (s.tail) hipLaunchKernelGGL((ln_bwd_rows_kernel<T, LPR, NV, true>), dim3(groups), dim3(256), 0, st, a);
         else hipLaunchKernelGGL((ln_bwd_rows_kernel<T, LPR, NV, false>), dim3(groups), dim3(256), 0, st, a);
@@ -73,38 +78,45 @@ void ln_launch_rows(const LnArgs& a, const LnShape& s, bool bwd, int groups, hip
     }
     // several rows a lane only where that leaves the chip full: short calls want their rows spread out
     if (U > 1 && a.rows >= (int64_t)RPB * U * 512) {
-        const int g = (int)(cdiv64(a.rows, RPB * U) < 8192 ? cdiv64(a.rows, RPB * U) : 8192);
+        const int g = (int)(cdiv64(a.rows, RPB * U) < LN_GRID ? cdiv64(a.rows, RPB * U) : LN_GRID);
         if (s.tail) hipLaunchKernelGGL((ln_fwd_rows_kernel<T, LPR, NV, U, true>), dim3(g), dim3(256), 0, st, a);
         else hipLaunchKernelGGL((ln_fwd_rows_kernel<T, LPR, NV, U, false>), dim3(g), dim3(256), 0, st, a);
     } else {
-        const int g = (int)(cdiv64(a.rows, RPB) < 8192 ? cdiv64(a.rows, RPB) : 8192);
+        const int g = (int)(cdiv64(a.rows, RPB) < LN_GRID ? cdiv64(a.rows, RPB) : LN_GRID);
         if (s.tail) hipLaunchKernelGGL((ln_fwd_rows_kernel<T, LPR, NV, 1, true>), dim3(g), dim3(256), 0, st, a);
         else hipLaunchKernelGGL((ln_fwd_rows_kernel<T, LPR, NV, 1, false>), dim3(g), dim3(256), 0, st, a);
     }
 }
 template <typename T, int W, int NV>
-void ln_launch_wide(const LnArgs& a, bool bwd, int groups, hipStream_t st) {
-    if (bwd) hipLaunchKernelGGL((ln_bwd_wide_kernel<T, W, NV>), dim3(groups), dim3(W * 64), 0, st, a);
-    else hipLaunchKernelGGL((ln_fwd_wide_kernel<T, W, NV>), dim3((int)(a.rows < 8192 ? a.rows : 8192)), dim3(W * 64), 0, st, a);
+void ln_launch_wide(const LnArgs& a, const LnShape& s, bool bwd, int groups, hipStream_t st) {
+    if (bwd) {
+        if (s.tail) hipLaunchKernelGGL((ln_bwd_wide_kernel<T, W, NV, true>), dim3(groups), dim3(W * 64), 0, st, a);
+        else hipLaunchKernelGGL((ln_bwd_wide_kernel<T, W, NV, false>), dim3(groups), dim3(W * 64), 0, st, a);
+        return;
+    }
+    const int g = (int)(a.rows < LN_GRID * 4 / W ? a.rows : LN_GRID * 4 / W);
+    if (s.tail) hipLaunchKernelGGL((ln_fwd_wide_kernel<T, W, NV, true>), dim3(g), dim3(W * 64), 0, st, a);
+    else hipLaunchKernelGGL((ln_fwd_wide_kernel<T, W, NV, false>), dim3(g), dim3(W * 64), 0, st, a);
 }
 template <typename T>
 void ln_launch(const LnArgs& a, const LnShape& s, bool bwd, int groups, hipStream_t st) {
-    constexpr bool F = sizeof(T) == 4;                    // bf16 vectors are twice as long: half the count
+    constexpr int V = sizeof(T) == 4 ? 2 : 1;             // vectors of 8 columns
     if (s.lpr) {
         if (s.lpr == 4) ln_launch_rows<T, 4, 1>(a, s, bwd, groups, st);
         else if (s.lpr == 8) ln_launch_rows<T, 8, 1>(a, s, bwd, groups, st);
         else if (s.lpr == 16) ln_launch_rows<T, 16, 1>(a, s, bwd, groups, st);
         else if (s.lpr == 32) ln_launch_rows<T, 32, 1>(a, s, bwd, groups, st);
         else if (s.nv == 1) ln_launch_rows<T, 64, 1>(a, s, bwd, groups, st);
-        else if (s.nv == 2) ln_launch_rows<T, 64, 2>(a, s, bwd, groups, st);
-        else ln_launch_rows<T, 64, F ? 4 : 2>(a, s, bwd, groups, st);
+        else ln_launch_rows<T, 64, V>(a, s, bwd, groups, st);
+    } else if (s.waves == 2) {
+        ln_launch_wide<T, 2, V>(a, s, bwd, groups, st);
     } else if (s.waves == 4) {
-        if (s.nv <= (F ? 2 : 1)) ln_launch_wide<T, 4, F ? 2 : 1>(a, bwd, groups, st);
-        else ln_launch_wide<T, 4, F ? 4 : 2>(a, bwd, groups, st);
+        ln_launch_wide<T, 4, V>(a, s, bwd, groups, st);
     } else if (s.waves == 8) {
-        ln_launch_wide<T, 8, F ? 4 : 2>(a, bwd, groups, st);
+        ln_launch_wide<T, 8, V>(a, s, bwd, groups, st);
     } else if (s.waves == 16) {
-        ln_launch_wide<T, 16, F ? 4 : 2>(a, bwd, groups, st);
+        if (s.nv == V) ln_launch_wide<T, 16, V>(a, s, bwd, groups, st);
+        else ln_launch_wide<T, 16, 2 * V>(a, s, bwd, groups, st);
     } else if (bwd) {
         if (a.y) hipLaunchKernelGGL((ln_bwd_long_kernel<T>), dim3((int)(a.rows < 2048 ? a.rows : 2048)), dim3(1024), 0, st, a);
         if (a.partial) hipLaunchKernelGGL((ln_cols_kernel<T>), dim3((a.C + 255) / 256, groups), dim3(256), 0, st, a);
@@ -379,7 +391,7 @@ int dvae_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_
         DVAE_CHECK_LAUNCH("layer_norm_bwd");
     }
     if (sums) {
-        hipLaunchKernelGGL(ln_reduce_kernel, dim3((unsigned)cdiv64(2LL * C, 64)), dim3(256), 0, S(st), (const float*)workspace,
+        hipLaunchKernelGGL(ln_reduce_kernel, dim3((unsigned)cdiv64(2LL * C, 64)), dim3(1024), 0, S(st), (const float*)workspace,
                            rows ? groups : 0, C, dgamma, dbeta);
         DVAE_CHECK_LAUNCH("layer_norm_bwd");
     }

@@ -31,21 +31,18 @@ template <> struct LnVec<bf16> {
 
 // N values at p[0 .. N), of which `left` exist; what does not exist reads as zero and is not touched in memory.
 template <typename T, bool TAIL>
-__device__ inline void ln_load(const T* p, int left, float (&v)[LnVec<T>::N]) {
+__device__ inline typename LnVec<T>::V ln_load(const T* p, int left) {
     constexpr int N = LnVec<T>::N;
-    if (left >= N) {
-        const typename LnVec<T>::V r = *reinterpret_cast<const typename LnVec<T>::V*>(p);
+    if (left >= N) return *reinterpret_cast<const typename LnVec<T>::V*>(p);
+    typename LnVec<T>::V r;
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = (float)r[i];
-    } else {
+    for (int i = 0; i < N; ++i) r[i] = (T)0.f;
+    if (TAIL) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = 0.f;
-        if (TAIL) {
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (i < left) v[i] = (float)p[i];
-        }
+        for (int i = 0; i < N; ++i)
+            if (i < left) r[i] = p[i];
     }
+    return r;
 }
 template <typename T, bool TAIL>
 __device__ inline void ln_store(T* p, int left, const float (&v)[LnVec<T>::N]) {
@@ -61,18 +58,56 @@ __device__ inline void ln_store(T* p, int left, const float (&v)[LnVec<T>::N]) {
             if (i < left) p[i] = (T)v[i];
     }
 }
+// A distance from the mean for element i of a vector of which `left` elements exist, 0 for the others.  Without a tail a
+// vector exists whole or not at all, and a mean of 0 does it for all of an absent one.
+template <bool TAIL, int N>
+__device__ inline float ln_mean_of(float mean, int left) { return TAIL || left >= N ? mean : 0.f; }
+template <bool TAIL>
+__device__ inline float ln_only(float v, int i, int left) { return !TAIL || i < left ? v : 0.f; }
 // gamma / beta (fp32), N of the columns from c on
 template <int N>
 __device__ inline void ln_param(const float* p, int c, int C, float missing, float (&v)[N]) {
+    if (p && c + N <= C) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = p && c + i < C ? p[c + i] : missing;
+        for (int k = 0; k < N; k += 4) {
+            const LnVec<float>::V r = *reinterpret_cast<const LnVec<float>::V*>(p + c + k);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[k + i] = r[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = p && c + i < C ? p[c + i] : missing;
+    }
 }
 
-// Sum over the LPR lanes of a row; result in all of them.
+// Keeps the compiler from holding what it derived from a vector in registers instead of the vector itself (twice the size and more).
+template <typename V>
+__device__ inline void ln_forget(V& v) {
+    u32x4 r = __builtin_bit_cast(u32x4, v);
+    asm volatile("" : "+v"(r));
+    v = __builtin_bit_cast(V, r);
+}
+
+// Sum over the LPR lanes of a row, in all of them: neighbours, pairs of pairs, halves of 8 and of 16 by data-parallel-primitive
+// moves, then the rows of 16 by lane swaps.  Every step adds the same two numbers in either lane, so all lanes agree to the bit.
+template <int CTRL>
+__device__ inline float dpp_add(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
 template <int LPR>
 __device__ inline float row_sum(float v) {
-#pragma unroll
-    for (int o = LPR >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    if (LPR > 1) v = dpp_add<0xB1>(v);                   // quad_perm 1,0,3,2
+    if (LPR > 2) v = dpp_add<0x4E>(v);                   // quad_perm 2,3,0,1
+    if (LPR > 4) v = dpp_add<0x141>(v);                  // row_half_mirror
+    if (LPR > 8) v = dpp_add<0x140>(v);                  // row_mirror
+    if (LPR > 16) {
+        const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false));
+        v = __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+    }
+    if (LPR > 32) {
+        const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false));
+        v = __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+    }
     return v;
 }
 // Sum over a workgroup of W waves; result in every thread.  `red` is W floats, free again after the second barrier.
@@ -105,12 +140,11 @@ __device__ inline void wg_sum2(float& a, float& b, float (*red)[W]) {
 struct LnStat {
     float off, inv;
 };
-__device__ inline LnStat ln_stat(float sum_d, float sum_d2, float c, float eps) {
+__device__ inline LnStat ln_stat(float sum_d, float sum_d2, float inv_c, float eps) {
     LnStat t;
-    t.off = sum_d / c;
-    const float v = sum_d2 / c - t.off * t.off;
-    t.inv = 1.f / sqrtf(fmaxf(v, 0.f) + eps);
-    if (v != v) t.inv = v;                               // fmaxf would hide a NaN
+    t.off = sum_d * inv_c;
+    const float v = sum_d2 * inv_c - t.off * t.off;
+    t.inv = rsqrtf((v < 0.f ? 0.f : v) + eps);           // a NaN stays one
     return t;
 }
 
@@ -142,53 +176,55 @@ __global__ __launch_bounds__(256) void ln_fwd_rows_kernel(LnArgs a) {
         ln_param<N>(a.gamma, c, a.C, 1.f, ga[j]);
         ln_param<N>(a.beta, c, a.C, 0.f, be[j]);
     }
-    const float cf = (float)a.C;
+    const float inv_c = 1.f / (float)a.C;
     for (long r0 = (long)blockIdx.x * RPB * U; r0 < a.rows; r0 += (long)gridDim.x * RPB * U) {
-        float v[U][NV][N];
+        typename LnVec<T>::V v[U][NV];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const long r = r0 + u * RPB + slot;
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const int c = (j * LPR + lane) * N;
-                ln_load<T, TAIL>(x + r * a.xs + c, r < a.rows ? a.C - c : 0, v[u][j]);
+                v[u][j] = ln_load<T, TAIL>(x + r * a.xs + c, r < a.rows ? a.C - c : 0);
             }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const long r = r0 + u * RPB + slot;
+            float d[NV][N];
             float s = 0.f, q = 0.f, e = 0.f;
 #pragma unroll
             for (int j = 0; j < NV; ++j)
 #pragma unroll
-                for (int i = 0; i < N; ++i) s += v[u][j][i];
-            const float mean = row_sum<LPR>(s) / cf;
+                for (int i = 0; i < N; ++i) s += (float)v[u][j][i];
+            const float mean = row_sum<LPR>(s) * inv_c;
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const int left = a.C - (j * LPR + lane) * N;
+                const float m = ln_mean_of<TAIL, N>(mean, left);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const float d = v[u][j][i] - mean;
-                    v[u][j][i] = d;
-                    e += i < left ? d : 0.f;
-                    q += i < left ? d * d : 0.f;
+                    d[j][i] = ln_only<TAIL>((float)v[u][j][i] - m, i, left);
+                    e += d[j][i];
+                    q += d[j][i] * d[j][i];
                 }
             }
-            const LnStat t = ln_stat(row_sum<LPR>(e), row_sum<LPR>(q), cf, a.eps);
+            const LnStat t = ln_stat(row_sum<LPR>(e), row_sum<LPR>(q), inv_c, a.eps);
             if (r < a.rows) {
                 if (lane == 0 && a.mean) { a.mean[r] = mean + t.off; a.invstd[r] = t.inv; }
 #pragma unroll
                 for (int j = 0; j < NV; ++j) {
                     const int c = (j * LPR + lane) * N;
 #pragma unroll
-                    for (int i = 0; i < N; ++i) v[u][j][i] = (v[u][j][i] - t.off) * t.inv * ga[j][i] + be[j][i];
-                    ln_store<T, TAIL>(y + r * a.ys + c, a.C - c, v[u][j]);
+                    for (int i = 0; i < N; ++i) d[j][i] = (d[j][i] - t.off) * t.inv * ga[j][i] + be[j][i];
+                    ln_store<T, TAIL>(y + r * a.ys + c, a.C - c, d[j]);
                 }
             }
         }
     }
 }
 
+// The next row's data is in flight, as it lies in memory, while a row is worked on.
 template <typename T, int LPR, int NV, bool TAIL>
 __global__ __launch_bounds__(256) void ln_bwd_rows_kernel(LnArgs a) {
     constexpr int N = LnVec<T>::N, RPB = 256 / LPR;
@@ -205,14 +241,15 @@ __global__ __launch_bounds__(256) void ln_bwd_rows_kernel(LnArgs a) {
     }
     const float inv_c = 1.f / (float)a.C;
     const long step = (long)gridDim.x * RPB;
-    float nx[NV][N], nd[NV][N], nm, ni;                  // the next row's data, in flight while this row is worked on
+    typename LnVec<T>::V nx[NV], nd[NV];
+    float nm, ni;
     auto fetch = [&](long r) {
         const bool in = r < a.rows;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int c = (j * LPR + lane) * N;
-            ln_load<T, TAIL>(x + r * a.xs + c, in ? a.C - c : 0, nx[j]);
-            ln_load<T, TAIL>(dy + r * a.ds + c, in ? a.C - c : 0, nd[j]);
+            nx[j] = ln_load<T, TAIL>(x + r * a.xs + c, in ? a.C - c : 0);
+            nd[j] = ln_load<T, TAIL>(dy + r * a.ds + c, in ? a.C - c : 0);
         }
         nm = in ? a.mean[r] : 0.f;
         ni = in ? a.invstd[r] : 0.f;
@@ -220,33 +257,37 @@ __global__ __launch_bounds__(256) void ln_bwd_rows_kernel(LnArgs a) {
     fetch((long)blockIdx.x * RPB + slot);
     for (long r0 = (long)blockIdx.x * RPB; r0 < a.rows; r0 += step) {
         const long r = r0 + slot;
-        float xh[NV][N], g[NV][N];
+        typename LnVec<T>::V vx[NV], vd[NV];
         const float mean = nm, inv = ni;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) { vx[j] = nx[j]; vd[j] = nd[j]; }
+        fetch(r + step);
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int left = a.C - (j * LPR + lane) * N;
+            const float m = ln_mean_of<TAIL, N>(mean, left);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float h = (nx[j][i] - mean) * inv, d = nd[j][i];
-                dg[j][i] += i < left ? d * h : 0.f;
+                const float h = ln_only<TAIL>(((float)vx[j][i] - m) * inv, i, left), d = (float)vd[j][i], g = d * ga[j][i];
+                dg[j][i] += d * h;
                 db[j][i] += d;
-                const float gi = d * ga[j][i];
-                xh[j][i] = h;
-                g[j][i] = gi;
-                s1 += gi;
-                s2 += i < left ? gi * h : 0.f;
+                s1 += g;
+                s2 += g * h;
             }
         }
-        fetch(r + step);
+        // dx = inv (g - c1 - h c2)
         const float c1 = row_sum<LPR>(s1) * inv_c, c2 = row_sum<LPR>(s2) * inv_c;
         if (r < a.rows && dx) {
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const int c = (j * LPR + lane) * N;
+                float o[N];
+                ln_forget(vx[j]);
+                ln_forget(vd[j]);
 #pragma unroll
-                for (int i = 0; i < N; ++i) g[j][i] = inv * (g[j][i] - c1 - xh[j][i] * c2);
-                ln_store<T, TAIL>(dx + r * a.ys + c, a.C - c, g[j]);
+                for (int i = 0; i < N; ++i) o[i] = inv * ((float)vd[j][i] * ga[j][i] - c1 - ((float)vx[j][i] - mean) * inv * c2);
+                ln_store<T, TAIL>(dx + r * a.ys + c, a.C - c, o);
             }
         }
     }
@@ -271,57 +312,70 @@ __global__ __launch_bounds__(256) void ln_bwd_rows_kernel(LnArgs a) {
     }
 }
 
-// ---- a row in a workgroup of W waves ------------------------------------------------------------------------------
-template <typename T, int W, int NV>
+// ---- a row in a workgroup of W waves, the next row's data in flight ---------------------------------------------------
+template <typename T, int W, int NV, bool TAIL>
 __global__ __launch_bounds__(W * 64) void ln_fwd_wide_kernel(LnArgs a) {
     constexpr int N = LnVec<T>::N;
     __shared__ float red[W], red2[2][W];
     const T* x = (const T*)a.x;
     T* y = (T*)a.y;
-    const float cf = (float)a.C;
-    for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        float v[NV][N];
+    const float inv_c = 1.f / (float)a.C;
+    float ga[NV][N], be[NV][N];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int c = (j * W * 64 + (int)threadIdx.x) * N;
+        ln_param<N>(a.gamma, c, a.C, 1.f, ga[j]);
+        ln_param<N>(a.beta, c, a.C, 0.f, be[j]);
+    }
+    typename LnVec<T>::V n[NV];
+    auto fetch = [&](long r) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int c = (j * W * 64 + (int)threadIdx.x) * N;
-            ln_load<T, true>(x + r * a.xs + c, a.C - c, v[j]);
+            n[j] = ln_load<T, TAIL>(x + r * a.xs + c, r < a.rows ? a.C - c : 0);
         }
+    };
+    fetch(blockIdx.x);
+    for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        float d[NV][N];
         float s = 0.f, q = 0.f, e = 0.f;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int i = 0; i < N; ++i) s += v[j][i];
-        const float mean = wg_sum<W>(s, red) / cf;
+            for (int i = 0; i < N; ++i) {
+                d[j][i] = (float)n[j][i];
+                s += d[j][i];
+            }
+        fetch(r + gridDim.x);
+        const float mean = wg_sum<W>(s, red) * inv_c;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int left = a.C - (j * W * 64 + (int)threadIdx.x) * N;
+            const float m = ln_mean_of<TAIL, N>(mean, left);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float d = v[j][i] - mean;
-                v[j][i] = d;
-                e += i < left ? d : 0.f;
-                q += i < left ? d * d : 0.f;
+                d[j][i] = ln_only<TAIL>(d[j][i] - m, i, left);
+                e += d[j][i];
+                q += d[j][i] * d[j][i];
             }
         }
         wg_sum2<W>(e, q, red2);
-        const LnStat t = ln_stat(e, q, cf, a.eps);
+        const LnStat t = ln_stat(e, q, inv_c, a.eps);
         if (threadIdx.x == 0 && a.mean) { a.mean[r] = mean + t.off; a.invstd[r] = t.inv; }
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int c = (j * W * 64 + (int)threadIdx.x) * N;
-            float ga[N], be[N];
-            ln_param<N>(a.gamma, c, a.C, 1.f, ga);
-            ln_param<N>(a.beta, c, a.C, 0.f, be);
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[j][i] = (v[j][i] - t.off) * t.inv * ga[i] + be[i];
-            ln_store<T, true>(y + r * a.ys + c, a.C - c, v[j]);
+            for (int i = 0; i < N; ++i) d[j][i] = (d[j][i] - t.off) * t.inv * ga[j][i] + be[j][i];
+            ln_store<T, TAIL>(y + r * a.ys + c, a.C - c, d[j]);
         }
     }
 }
 
-template <typename T, int W, int NV>
+template <typename T, int W, int NV, bool TAIL>
 __global__ __launch_bounds__(W * 64) void ln_bwd_wide_kernel(LnArgs a) {
     constexpr int N = LnVec<T>::N;
+    constexpr bool AHEAD = NV * N <= 8;                  // 16 columns a thread leave no registers for the next row
     __shared__ float red[2][W];
     const T *x = (const T*)a.x, *dy = (const T*)a.dy;
     T* dx = (T*)a.y;
@@ -333,29 +387,35 @@ __global__ __launch_bounds__(W * 64) void ln_bwd_wide_kernel(LnArgs a) {
         for (int i = 0; i < N; ++i) { dg[j][i] = 0.f; db[j][i] = 0.f; }
     }
     const float inv_c = 1.f / (float)a.C;
-    for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        float xh[NV][N], g[NV][N];
+    typename LnVec<T>::V nx[NV], nd[NV];
+    auto fetch = [&](long r) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int c = (j * W * 64 + (int)threadIdx.x) * N;
-            ln_load<T, true>(x + r * a.xs + c, a.C - c, xh[j]);
-            ln_load<T, true>(dy + r * a.ds + c, a.C - c, g[j]);
+            nx[j] = ln_load<T, TAIL>(x + r * a.xs + c, r < a.rows ? a.C - c : 0);
+            nd[j] = ln_load<T, TAIL>(dy + r * a.ds + c, r < a.rows ? a.C - c : 0);
         }
+    };
+    if (AHEAD) fetch(blockIdx.x);
+    for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        typename LnVec<T>::V vx[NV], vd[NV];
+        if (!AHEAD) fetch(r);
         const float mean = a.mean[r], inv = a.invstd[r];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) { vx[j] = nx[j]; vd[j] = nd[j]; }
+        if (AHEAD) fetch(r + gridDim.x);
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int left = a.C - (j * W * 64 + (int)threadIdx.x) * N;
+            const float m = ln_mean_of<TAIL, N>(mean, left);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float h = (xh[j][i] - mean) * inv, d = g[j][i];
-                dg[j][i] += i < left ? d * h : 0.f;
+                const float h = ln_only<TAIL>(((float)vx[j][i] - m) * inv, i, left), d = (float)vd[j][i], g = d * ga[j][i];
+                dg[j][i] += d * h;
                 db[j][i] += d;
-                const float gi = d * ga[j][i];
-                xh[j][i] = h;
-                g[j][i] = gi;
-                s1 += gi;
-                s2 += i < left ? gi * h : 0.f;
+                s1 += g;
+                s2 += g * h;
             }
         }
         wg_sum2<W>(s1, s2, red);
@@ -364,9 +424,12 @@ __global__ __launch_bounds__(W * 64) void ln_bwd_wide_kernel(LnArgs a) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int c = (j * W * 64 + (int)threadIdx.x) * N;
+            float o[N];
+            ln_forget(vx[j]);
+            ln_forget(vd[j]);
 #pragma unroll
-            for (int i = 0; i < N; ++i) g[j][i] = inv * (g[j][i] - c1 - xh[j][i] * c2);
-            ln_store<T, true>(dx + r * a.ys + c, a.C - c, g[j]);
+            for (int i = 0; i < N; ++i) o[i] = inv * ((float)vd[j][i] * ga[j][i] - c1 - ((float)vx[j][i] - mean) * inv * c2);
+            ln_store<T, TAIL>(dx + r * a.ys + c, a.C - c, o);
         }
     }
     if (!a.partial) return;
@@ -384,16 +447,16 @@ __global__ __launch_bounds__(W * 64) void ln_bwd_wide_kernel(LnArgs a) {
 template <typename T>
 __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(LnArgs a) {
     __shared__ float red[16], red2[2][16];
-    const float cf = (float)a.C;
+    const float inv_c = 1.f / (float)a.C;
     for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T* x = (const T*)a.x + r * a.xs;
         T* y = (T*)a.y + r * a.ys;
         float s = 0.f, q = 0.f, e = 0.f;
         for (int c = threadIdx.x; c < a.C; c += 1024) s += (float)x[c];
-        const float mean = wg_sum<16>(s, red) / cf;
+        const float mean = wg_sum<16>(s, red) * inv_c;
         for (int c = threadIdx.x; c < a.C; c += 1024) { const float d = (float)x[c] - mean; e += d; q += d * d; }
         wg_sum2<16>(e, q, red2);
-        const LnStat t = ln_stat(e, q, cf, a.eps);
+        const LnStat t = ln_stat(e, q, inv_c, a.eps);
         if (threadIdx.x == 0 && a.mean) { a.mean[r] = mean + t.off; a.invstd[r] = t.inv; }
         for (int c = threadIdx.x; c < a.C; c += 1024)
             y[c] = (T)(((float)x[c] - mean - t.off) * t.inv * (a.gamma ? a.gamma[c] : 1.f) + (a.beta ? a.beta[c] : 0.f));
@@ -440,28 +503,29 @@ __global__ __launch_bounds__(256) void ln_cols_kernel(LnArgs a) {
     out[a.C + c] = db;
 }
 
-// slabs [G][2][C] -> dgamma, dbeta: 64 columns a workgroup, its four waves take every fourth slab
-__global__ __launch_bounds__(256) void ln_reduce_kernel(const float* partial, int G, int C, float* dgamma, float* dbeta) {
-    __shared__ float red[4][64];
+// slabs [G][2][C] -> dgamma, dbeta: 64 columns a workgroup, its 16 waves take every 16th slab, eight loads in flight each
+__global__ __launch_bounds__(1024) void ln_reduce_kernel(const float* partial, int G, int C, float* dgamma, float* dbeta) {
+    __shared__ float red[16][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int e = blockIdx.x * 64 + lane;                // index into [2][C]
-    float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;        // four chains: their loads are in flight together
+    float s = 0.f;
     if (e < 2 * C) {
         const float* p = partial + e;
         const long st = 2L * C;
-        int g = wave;
-        for (; g + 12 < G; g += 16) {
-            s0 += p[g * st];
-            s1 += p[(g + 4) * st];
-            s2 += p[(g + 8) * st];
-            s3 += p[(g + 12) * st];
+        for (int g = wave; g < G; g += 128) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = g + 16 * i < G ? p[(g + 16 * i) * st] : 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += v[i];
         }
-        for (; g < G; g += 4) s0 += p[g * st];
     }
-    red[wave][lane] = (s0 + s1) + (s2 + s3);
+    red[wave][lane] = s;
     __syncthreads();
     if (wave == 0 && e < 2 * C) {
-        const float s = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s += red[i][lane];
         float* out = e < C ? dgamma : dbeta;
         if (out) out[e < C ? e : e - C] = s;
     }
