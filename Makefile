@@ -4,7 +4,7 @@ ARCH ?= gfx950
 PKG := d-vae_amd
 CSRC := $(PKG)/csrc
 LIB := $(PKG)/lib/libdvae_hip.so
-LEARN_HDRS := $(CSRC)/layer_norm.hpp $(CSRC)/newton_schulz.hpp
+LEARN_HDRS := $(CSRC)/layer_norm.hpp $(CSRC)/newton_schulz.hpp $(CSRC)/newton_schulz_small.hpp
 HDRS := $(filter-out $(LEARN_HDRS),$(wildcard $(CSRC)/*.hpp)) include/dvae_hip.h
 FLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -fno-gpu-rdc -Wall -Wno-unused-function -mllvm -pragma-unroll-threshold=1000000
 # no packed fp32 arithmetic in the kernels (the host pass does not know the feature and says so)

@@ -9,6 +9,7 @@
 #include "common.hpp"
 #include "layer_norm.hpp"
 #include "newton_schulz.hpp"
+#include "newton_schulz_small.hpp"
 
 using namespace dvae;
 
@@ -194,6 +195,54 @@ inline long ns_triangles(int P, int ts) {
     return t * (t + 1) / 2;
 }
 
+void ns_job(const dvae_matrix& m, int scale_rule, NsJob& j) {
+    j = NsJob{};
+    j.x = m.x; j.out = m.out; j.mom = m.momentum;
+    j.xs = m.x_stride; j.os = m.out_stride;
+    j.m = (int)m.rows; j.n = (int)m.cols;
+    j.vec = m.vector ? 1 : 0;
+    const double r = (double)j.m, c = (double)j.n;
+    j.scale = (float)(scale_rule == DVAE_MUON_RMS ? 0.2 * sqrt(fmax(r, c)) : sqrt(fmax(1.0, r / c)));
+}
+
+// Whether every matrix of a call fits the one-launch kernel.  One that does not makes the whole call go through the batched
+// phases, where small matrices ride along for next to nothing.
+bool ns_all_small(const dvae_matrix* mats, int count) {
+    for (int i = 0; i < count; ++i) {
+        const int64_t p = mats[i].rows < mats[i].cols ? mats[i].rows : mats[i].cols, q = mats[i].rows < mats[i].cols ? mats[i].cols : mats[i].rows;
+        if (mats[i].vector ? mats[i].rows * mats[i].cols > NS_SMALL_VEC : p > NS_SMALL_P || q > NS_SMALL_Q) return false;
+    }
+    return true;
+}
+
+template <typename T, bool MUON>
+int ns_run_small(const char* what, const dvae_matrix* mats, int count, int scale_rule, const NsArgs& g, int steps, hipStream_t st) {
+    static LdsOptIn opt[3];
+    NsSmallArgs a{};
+    a.eps = g.eps; a.a = g.a; a.b = g.b; a.c = g.c; a.mu = g.mu; a.nu = g.nu; a.lr = g.lr; a.decay = g.decay;
+    a.nesterov = g.nesterov; a.steps = steps;
+    for (int i = 0; i < count; i += NS_SMALL_JOBS) {
+        const int some = count - i < NS_SMALL_JOBS ? count - i : NS_SMALL_JOBS;
+        int q = 1;
+        for (int k = 0; k < some; ++k) {
+            ns_job(mats[i + k], scale_rule, a.jobs[k]);
+            if (!a.jobs[k].vec) q = fmax(q, fmax(a.jobs[k].m, a.jobs[k].n));
+        }
+        const int lds = (int)sizeof(NsSmallLds);
+#define NS_SMALL_LAUNCH(NB)                                                                                          \
+    do {                                                                                                             \
+        opt[NB - 1].ensure((const void*)ns_small_kernel<T, MUON, NB>, lds);                                          \
+        hipLaunchKernelGGL((ns_small_kernel<T, MUON, NB>), dim3(some), dim3(512), lds, st, a);                       \
+    } while (0)
+        if (q <= 256) NS_SMALL_LAUNCH(1);
+        else if (q <= 512) NS_SMALL_LAUNCH(2);
+        else NS_SMALL_LAUNCH(3);
+#undef NS_SMALL_LAUNCH
+        DVAE_CHECK_LAUNCH(what);
+    }
+    return DVAE_OK;
+}
+
 int ns_plan(const char* what, const dvae_matrix* mats, int count, int scale_rule, NsPlan& p) {
     p.njobs = count;
     p.jp = (count + 1 + 63) / 64 * 64;
@@ -201,7 +250,7 @@ int ns_plan(const char* what, const dvae_matrix* mats, int count, int scale_rule
     std::vector<int> first((size_t)NS_PHASES * p.jp, INT_MAX);
     // Tiles of 128 read half as much LDS per product as tiles of 64, and want enough of them: the larger tile is taken
     // where its tiles alone give every CU one.
-    long big_apply = 0, big_sym = 0, sym64 = 0, lines64 = 0;
+    long big_apply = 0, big_sym = 0, sym64 = 0, lines64 = 0, longest = 0;
     for (int i = 0; i < count; ++i) {
         const dvae_matrix& m = mats[i];
         if (m.vector) continue;
@@ -210,6 +259,7 @@ int ns_plan(const char* what, const dvae_matrix* mats, int count, int scale_rule
         big_sym += ns_triangles((int)P, 128);
         sym64 += ns_triangles((int)P, 64);
         lines64 += ns_triangles((int)P, 64) * (Q / 32);
+        longest = longest > Q / 32 ? longest : Q / 32;
         p.matrices = true;
     }
     p.apply_ts = big_apply >= 256 ? 128 : 64;
@@ -219,20 +269,17 @@ int ns_plan(const char* what, const dvae_matrix* mats, int count, int scale_rule
     if (p.gram_ts == 64 && sym64 < 512) {
         p.kc = (int)((lines64 + 511) / 512);
         if (p.kc < 4) p.kc = 4;
+        if (p.kc < (longest + 31) / 32) p.kc = (int)((longest + 31) / 32);      // at most 32 of a tile, which one workgroup adds up
+        p.kc = (p.kc + 1) & ~1;
     }
     long off = 0, part = 0;
     for (int i = 0; i < count; ++i) {
         const dvae_matrix& m = mats[i];
         NsJob& j = jobs[i];
-        j.x = m.x; j.out = m.out; j.mom = m.momentum;
-        j.xs = m.x_stride; j.os = m.out_stride;
-        j.m = (int)m.rows; j.n = (int)m.cols;
-        j.vec = m.vector ? 1 : 0;
+        ns_job(m, scale_rule, j);
         const long chunks = ((long)j.m * j.n + NS_CHUNK - 1) / NS_CHUNK;
         j.nchunk = (int)(chunks < 1024 ? chunks : 1024);
         j.part = (int)part;
-        const double r = (double)j.m, c = (double)j.n;
-        j.scale = (float)(scale_rule == DVAE_MUON_RMS ? 0.2 * sqrt(fmax(r, c)) : sqrt(fmax(1.0, r / c)));
         for (int f = 0; f < NS_PHASES; ++f) {
             if (p.total[f] > INT_MAX / 2) DVAE_FAIL(DVAE_EINVAL, "%s: too much work for one call", what);
             first[(size_t)f * p.jp + i] = (int)p.total[f];
@@ -404,6 +451,7 @@ size_t dvae_newton_schulz_workspace_bytes(const dvae_matrix* mats, int count) {
         for (int i = 0; i < count; ++i)
             if (mats[i].rows <= 0 || mats[i].cols <= 0 || mats[i].rows > (1 << 30) || mats[i].cols > (1 << 30) ||
                 mats[i].rows * mats[i].cols >= (1LL << 31)) return 0;
+        if (ns_all_small(mats, count)) return 256;        // not used; the least there is
         NsPlan p;
         return ns_plan("newton_schulz", mats, count, DVAE_MUON_SPECTRAL, p) ? 0 : p.bytes;
     } catch (...) {
@@ -420,13 +468,18 @@ int dvae_newton_schulz(const dvae_matrix* mats, int count, const double* coeffic
         for (int i = 0; i < count; ++i)
             if (mats[i].vector) DVAE_FAIL(DVAE_EINVAL, "newton_schulz: matrix %d is marked as a vector", i);
         if (count == 0) return DVAE_OK;
-        NsPlan p;
-        if ((rc = ns_plan("newton_schulz", mats, count, DVAE_MUON_SPECTRAL, p))) return rc;
-        if ((rc = ns_workspace_check("newton_schulz", workspace, workspace_bytes, p.bytes))) return rc;
         NsArgs g{};
         g.ws = (char*)workspace;
         g.a = (float)coefficients[0]; g.b = (float)coefficients[1]; g.c = (float)coefficients[2];
         g.eps = eps;
+        const bool small = ns_all_small(mats, count);
+        if (small && (rc = ns_workspace_check("newton_schulz", workspace, workspace_bytes, 256))) return rc;
+        if (small)
+            return dtype == DVAE_F32 ? ns_run_small<float, false>("newton_schulz", mats, count, DVAE_MUON_SPECTRAL, g, steps, S(st))
+                                     : ns_run_small<bf16, false>("newton_schulz", mats, count, DVAE_MUON_SPECTRAL, g, steps, S(st));
+        NsPlan p;
+        if ((rc = ns_plan("newton_schulz", mats, count, DVAE_MUON_SPECTRAL, p))) return rc;
+        if ((rc = ns_workspace_check("newton_schulz", workspace, workspace_bytes, p.bytes))) return rc;
         return dtype == DVAE_F32 ? ns_run<float, false>("newton_schulz", p, g, steps, S(st))
                                  : ns_run<bf16, false>("newton_schulz", p, g, steps, S(st));
     } catch (...) {
@@ -444,15 +497,19 @@ int dvae_muon_step(const dvae_matrix* mats, int count, double lr, double momentu
         if (!(momentum >= 0.0 && momentum < 1.0) || !(lr >= 0.0) || !(weight_decay >= 0.0) || !isfinite(lr * weight_decay))
             DVAE_FAIL(DVAE_EINVAL, "muon_step: lr %g, momentum %g, weight decay %g", lr, momentum, weight_decay);
         if (count == 0) return DVAE_OK;
-        NsPlan p;
-        if ((rc = ns_plan("muon_step", mats, count, scale_rule, p))) return rc;
-        if ((rc = ns_workspace_check("muon_step", workspace, workspace_bytes, p.bytes))) return rc;
         NsArgs g{};
         g.ws = (char*)workspace;
         g.a = (float)coefficients[0]; g.b = (float)coefficients[1]; g.c = (float)coefficients[2];
         g.eps = eps;
         g.mu = (float)momentum; g.nu = (float)(1.0 - momentum); g.nesterov = nesterov; g.lr = (float)lr;
         g.decay = (float)(1.0 - lr * weight_decay);
+        if (ns_all_small(mats, count)) {
+            if ((rc = ns_workspace_check("muon_step", workspace, workspace_bytes, 256))) return rc;
+            return ns_run_small<float, true>("muon_step", mats, count, scale_rule, g, steps, S(st));
+        }
+        NsPlan p;
+        if ((rc = ns_plan("muon_step", mats, count, scale_rule, p))) return rc;
+        if ((rc = ns_workspace_check("muon_step", workspace, workspace_bytes, p.bytes))) return rc;
         return ns_run<float, true>("muon_step", p, g, steps, S(st));
     } catch (...) {
         DVAE_FAIL(DVAE_EINVAL, "muon_step: out of host memory");

@@ -11,8 +11,9 @@
 // hh + hl + lh, summed in fp32: the errors of an fp32 product at 3/16 of its time.  fp16's range is met by fixed scales: with
 // the coefficients' bounds checked on the host, |X| <= 2, |A| <= 4 and |B| <= 7, held as 2^14 X, 2^13 A and 2^13 B.
 //
-// Layout.  A plane pair of an R x K operand holds, per row, lines of 128 bytes: 32 h's, then the 32 l's of the same
-// columns.  R and K are padded to 64 with zeros, which the products keep zero.  X is kept with its transpose (two copies,
+// Layout.  A plane pair of an R x K operand is made of lines of 128 bytes: 32 h's of a row, then the 32 l's of the same
+// columns.  The lines of the R rows follow each other, then those of the next 32 columns: what a tile reads or writes at a time
+// is one run of memory.  R and K are padded to 64 with zeros, which the products keep zero.  X is kept with its transpose (two copies,
 // taken in turn), so that every product reads both operands along its contraction and every store writes whole lines.
 #pragma once
 #include "common.hpp"
@@ -22,6 +23,14 @@ namespace dvae {
 using f16 = _Float16;
 using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
 using f16x2 = __attribute__((ext_vector_type(2))) _Float16;
+
+// Pointers that come out of the job table are told to be global memory: the compiler cannot know, and its flat accesses count
+// as LDS traffic too, which makes every wait for a fragment one for the loads in flight as well.
+#define DVAE_GLOBAL __attribute__((address_space(1)))
+using gbytes = DVAE_GLOBAL char*;
+using cgbytes = const DVAE_GLOBAL char*;
+template <typename T>
+__device__ inline DVAE_GLOBAL T* as_global(const void* p) { return (DVAE_GLOBAL T*)(uintptr_t)p; }
 
 constexpr float NS_SX = 16384.f, NS_SA = 8192.f, NS_SB = 8192.f;
 
@@ -99,20 +108,29 @@ __device__ inline int ns_swizzle(int id, int total) {
 
 struct NsPlanes {
     int P, Q;
-    char *x, *xt[2], *a, *b;
+    gbytes x, xt0, xt1, a, b;
     __device__ NsPlanes(const NsArgs& g, const NsJob& j) {
         P = ns_pad(min(j.m, j.n));
         Q = ns_pad(max(j.m, j.n));
         const long pq = 4L * P * Q;
-        x = g.ws + j.off;
-        xt[0] = x + pq;
-        xt[1] = x + 2 * pq;
+        x = as_global<char>(g.ws) + j.off;
+        xt0 = x + pq;
+        xt1 = x + 2 * pq;
         a = x + 3 * pq;
         b = a + 4L * P * P;
     }
+    __device__ gbytes xt(int which) const { return which ? xt1 : xt0; }
 };
 
+// A value that is about to be split is rounded to fp32 for good.  Left to itself the compiler converts a product to fp16 now
+// from its rounded value and now, fused, from its exact one; at a tie the h that is stored and the h that l is the rest of are
+// then two neighbours, and the pair is off by 2^-11.
+__device__ inline float ns_rounded(float v) {
+    asm("" : "+v"(v));
+    return v;
+}
 __device__ inline unsigned ns_split(float v) {           // low half: h, high half: l
+    v = ns_rounded(v);
     const f16 h = (f16)v;
     const f16 l = (f16)(v - (float)h);
     const f16x2 r = {h, l};
@@ -132,7 +150,8 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs g) {
     int chunk;
     const NsJob j = g.jobs[ns_find(g, NS_NORM, blockIdx.x, chunk)];
     const long n = (long)j.m * j.n;
-    const T* x = (const T*)j.x;
+    const auto x = as_global<const T>(j.x);
+    const auto mom = as_global<float>(j.mom), par = as_global<float>(j.out);
     double s = 0.0;
     for (long base = (long)chunk * NS_CHUNK; base < n; base += (long)j.nchunk * NS_CHUNK) {
         float v[16];
@@ -148,16 +167,16 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs g) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const long e = base + i * 256 + threadIdx.x;
-                m[i] = e < n ? j.mom[e] : 0.f;
-                p[i] = e < n && j.vec ? ((float*)j.out)[e] : 0.f;
+                m[i] = e < n ? mom[e] : 0.f;
+                p[i] = e < n && j.vec ? par[e] : 0.f;
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const long e = base + i * 256 + threadIdx.x;
                 const float mi = ns_momentum(g, v[i], m[i]);
-                if (e < n) j.mom[e] = mi;
+                if (e < n) mom[e] = mi;
                 v[i] = ns_update(g, v[i], mi);
-                if (e < n && j.vec) ((float*)j.out)[e] = p[i] * g.decay - g.lr * v[i];
+                if (e < n && j.vec) par[e] = p[i] * g.decay - g.lr * v[i];
             }
         }
 #pragma unroll
@@ -196,8 +215,8 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsArgs g) {
         float v = 0.f;
         if (r < j.m && c < j.n) {
             const long e = (long)r * j.xs + c;
-            v = (float)((const T*)j.x)[e];
-            if (MUON) v = ns_update(g, v, j.mom[e]);
+            v = (float)as_global<const T>(j.x)[e];
+            if (MUON) v = ns_update(g, v, as_global<float>(j.mom)[e]);
             v = (float)((double)v * inv);
         }
         tile[i * 4 + wave][lane] = ns_split(v);
@@ -206,8 +225,8 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsArgs g) {
     // a thread writes 16 columns of a row: first in the source's orientation, then in the other
 #pragma unroll
     for (int flip = 0; flip < 2; ++flip) {
-        char* dst = flip ? (tall ? w.x : w.xt[0]) : (tall ? w.xt[0] : w.x);
-        const long pitch = 4L * ns_pad(flip ? j.m : j.n);
+        gbytes dst = flip ? (tall ? w.x : w.xt0) : (tall ? w.xt0 : w.x);
+        const long rows = ns_pad(flip ? j.n : j.m);
         const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 16;
         unsigned h[8], l[8];
 #pragma unroll
@@ -218,24 +237,29 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsArgs g) {
             l[i] = (u0 >> 16) | (u1 & 0xffff0000u);
         }
         const int row = (flip ? c0 : r0) + r, col = (flip ? r0 : c0) + c;
-        char* p = dst + row * pitch + (col >> 5) * 128 + (col & 31) * 2;
-        *reinterpret_cast<u32x4*>(p) = u32x4{h[0], h[1], h[2], h[3]};
-        *reinterpret_cast<u32x4*>(p + 16) = u32x4{h[4], h[5], h[6], h[7]};
-        *reinterpret_cast<u32x4*>(p + 64) = u32x4{l[0], l[1], l[2], l[3]};
-        *reinterpret_cast<u32x4*>(p + 80) = u32x4{l[4], l[5], l[6], l[7]};
+        gbytes p = dst + ((col >> 5) * rows + row) * 128 + (col & 31) * 2;
+        *(DVAE_GLOBAL u32x4*)(p) = u32x4{h[0], h[1], h[2], h[3]};
+        *(DVAE_GLOBAL u32x4*)(p + 16) = u32x4{h[4], h[5], h[6], h[7]};
+        *(DVAE_GLOBAL u32x4*)(p + 64) = u32x4{l[0], l[1], l[2], l[3]};
+        *(DVAE_GLOBAL u32x4*)(p + 80) = u32x4{l[4], l[5], l[6], l[7]};
     }
 }
 
 // ---- the products ----------------------------------------------------------------------------------------------------
 // C[i][k] = sum over c of L[i][c] R[k][c] for a TS x TS tile: four waves, a quarter tile each, 32x32x16 MFMAs.  Two LDS
-// stages of one line (32 columns) per row; the next line's loads are in flight in registers while a stage is multiplied.
-// A line's eight 16-byte chunks are stored at chunk ^ (row & 7): fragment reads (32 rows, one chunk) meet no bank twice.
+// stages of one line (32 columns) per row, one barrier a line: while one half of a line is multiplied, the fragments of the
+// other half are on their way from LDS, and the lines after next are on their way from memory in two sets of registers.
+// A line's eight 16-byte chunks are stored at chunk ^ (row / 2 & 7): of a fragment's rows any sixteen that are read at a time
+// meet the 64 banks once each.
 template <int TS>
 struct NsTile {
     static constexpr int S = TS / 64;                    // subtiles of a wave each way
     static constexpr int PASS = TS / 32;                 // passes of 256 threads over a stage of one operand
     static constexpr int BYTES = 2 * 2 * TS * 128;
     f32x16 acc[S][S];
+
+    struct Lines { u32x4 l[PASS], r[PASS]; };
+    struct Frags { f16x8 lh[S], ll[S], rh[S], rl[S]; };
 
     __device__ inline void zero() {
 #pragma unroll
@@ -246,70 +270,85 @@ struct NsTile {
                 for (int e = 0; e < 16; ++e) acc[i][k][e] = 0.f;
     }
 
-    // rows past lrows / rrows re-read the last one: their results are not stored
-    __device__ inline void run(const char* L, long lpitch, int l0, int lrows, const char* R, long rpitch, int r0, int rrows,
-                               int line0, int lines, char* smem) {
+    // MFMAs FROM to TO of the 3 S^2 of half a line
+    template <int FROM, int TO>
+    __device__ inline void multiply(const Frags& f) {
+#pragma unroll
+        for (int m = FROM; m < TO; ++m) {
+            const int w = m / (S * S), i = m / S % S, n = m % S;
+            acc[i][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w == 1 ? f.ll[i] : f.lh[i], w == 0 ? f.rl[n] : f.rh[n], acc[i][n], 0, 0, 0);
+        }
+    }
+    // `lines` is even; rows past lrows / rrows re-read the last one: their results are not stored
+    __device__ inline void run(cgbytes L, int lrows, int l0, cgbytes R, int rrows, int r0, int line0, int lines, char* smem) {
         const int tid = threadIdx.x, row = tid >> 3, chunk = tid & 7;
         const int lane = tid & 63, wave = tid >> 6;
-        const char *lp[PASS], *rp[PASS];
+        cgbytes lp[PASS], rp[PASS];
 #pragma unroll
         for (int i = 0; i < PASS; ++i) {
-            lp[i] = L + (long)min(l0 + i * 32 + row, lrows - 1) * lpitch + line0 * 128L + chunk * 16;
-            rp[i] = R + (long)min(r0 + i * 32 + row, rrows - 1) * rpitch + line0 * 128L + chunk * 16;
+            lp[i] = L + ((long)line0 * lrows + min(l0 + i * 32 + row, lrows - 1)) * 128 + chunk * 16;
+            rp[i] = R + ((long)line0 * rrows + min(r0 + i * 32 + row, rrows - 1)) * 128 + chunk * 16;
         }
-        u32x4 sl[PASS], sr[PASS];
-        auto fetch = [&]() {
+        Lines set[2];
+        int ahead = lines;
+        auto fetch = [&](Lines& s) {                      // the next line; past the last one, that one again
 #pragma unroll
             for (int i = 0; i < PASS; ++i) {
-                sl[i] = *reinterpret_cast<const u32x4*>(lp[i]);
-                sr[i] = *reinterpret_cast<const u32x4*>(rp[i]);
-                lp[i] += 128;
-                rp[i] += 128;
+                s.l[i] = *(const DVAE_GLOBAL u32x4*)lp[i];
+                s.r[i] = *(const DVAE_GLOBAL u32x4*)rp[i];
             }
-        };
-        const int put = row * 128 + ((chunk ^ (row & 7)) << 4);
-        auto stage = [&](int at) {
-            char* s = smem + at * (2 * TS * 128);
+            const bool more = --ahead > 0;
 #pragma unroll
             for (int i = 0; i < PASS; ++i) {
-                *reinterpret_cast<u32x4*>(s + i * 32 * 128 + put) = sl[i];
-                *reinterpret_cast<u32x4*>(s + TS * 128 + i * 32 * 128 + put) = sr[i];
+                lp[i] += more ? lrows * 128L : 0L;
+                rp[i] += more ? rrows * 128L : 0L;
             }
         };
-        const int lr = (wave >> 1) * (TS / 2) + (lane & 31), rr = (wave & 1) * (TS / 2) + (lane & 31), half = lane >> 5;
-        auto multiply = [&](int at) {
-            const char* sL = smem + at * (2 * TS * 128) + lr * 128;
-            const char* sR = smem + at * (2 * TS * 128) + TS * 128 + rr * 128;
-            const int sw = lane & 7;
+        const int put = row * 128 + ((chunk ^ (row >> 1 & 7)) << 4);
+        auto stage = [&](int at, const Lines& l) {
+            char* s = smem + at * (2 * TS * 128) + put;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                f16x8 lh[S], ll[S], rh[S], rl[S];
-                const int ch = ((k * 2 + half) ^ sw) << 4, cl = ((4 + k * 2 + half) ^ sw) << 4;
-#pragma unroll
-                for (int i = 0; i < S; ++i) {
-                    lh[i] = *reinterpret_cast<const f16x8*>(sL + i * 32 * 128 + ch);
-                    ll[i] = *reinterpret_cast<const f16x8*>(sL + i * 32 * 128 + cl);
-                    rh[i] = *reinterpret_cast<const f16x8*>(sR + i * 32 * 128 + ch);
-                    rl[i] = *reinterpret_cast<const f16x8*>(sR + i * 32 * 128 + cl);
-                }
-#pragma unroll
-                for (int i = 0; i < S; ++i)
-#pragma unroll
-                    for (int n = 0; n < S; ++n) {
-                        acc[i][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh[i], rl[n], acc[i][n], 0, 0, 0);
-                        acc[i][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ll[i], rh[n], acc[i][n], 0, 0, 0);
-                        acc[i][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh[i], rh[n], acc[i][n], 0, 0, 0);
-                    }
+            for (int i = 0; i < PASS; ++i) {
+                *reinterpret_cast<u32x4*>(s + i * 32 * 128) = l.l[i];
+                *reinterpret_cast<u32x4*>(s + TS * 128 + i * 32 * 128) = l.r[i];
             }
         };
-        fetch();
-        stage(0);
+        const int half = lane >> 5, sw = lane >> 1 & 7;
+        const char* sL = smem + ((wave >> 1) * (TS / 2) + (lane & 31)) * 128;
+        const char* sR = smem + TS * 128 + ((wave & 1) * (TS / 2) + (lane & 31)) * 128;
+        auto read = [&](Frags& f, int at, int k) {
+            const int ch = at * (2 * TS * 128) + (((k * 2 + half) ^ sw) << 4), cl = at * (2 * TS * 128) + (((4 + k * 2 + half) ^ sw) << 4);
+#pragma unroll
+            for (int i = 0; i < S; ++i) {
+                f.lh[i] = *reinterpret_cast<const f16x8*>(sL + i * 32 * 128 + ch);
+                f.rl[i] = *reinterpret_cast<const f16x8*>(sR + i * 32 * 128 + cl);
+            }
+#pragma unroll
+            for (int i = 0; i < S; ++i) {
+                f.ll[i] = *reinterpret_cast<const f16x8*>(sL + i * 32 * 128 + cl);
+                f.rh[i] = *reinterpret_cast<const f16x8*>(sR + i * 32 * 128 + ch);
+            }
+        };
+        Frags f0, f1;
+        fetch(set[0]);
+        fetch(set[1]);
+        stage(0, set[0]);
+        fetch(set[0]);
         __syncthreads();
-        for (int k = 0; k < lines; ++k) {
-            if (k + 1 < lines) fetch();
-            multiply(k & 1);
-            if (k + 1 < lines) stage((k + 1) & 1);
-            __syncthreads();
+        read(f0, 0, 0);
+        for (int k = 0; k < lines; k += 2) {
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+                read(f1, d, 1);
+                multiply<0, S * S>(f0);
+                stage(d ^ 1, set[d ^ 1]);
+                multiply<S * S, 3 * S * S>(f0);
+                fetch(set[d ^ 1]);
+                multiply<0, S * S>(f1);
+                __syncthreads();                          // this line's fragments are out, the next line is in
+                read(f0, d ^ 1, 0);
+                multiply<S * S, 3 * S * S>(f1);
+            }
         }
     }
 
@@ -320,9 +359,12 @@ struct NsTile {
     __device__ static inline int col_of(int k) { return ((threadIdx.x >> 6) & 1) * (TS / 2) + k * 32 + (threadIdx.x & 31); }
 };
 
+// the line of a row that holds column `col`, a multiple of 32
+__device__ inline gbytes ns_line(gbytes base, int rows, int row, int col) { return base + ((long)(col >> 5) * rows + row) * 128; }
+
 // A 32x32 subtile (already scaled) to plane pairs: along its rows at `dst` (through a per-wave LDS patch) and, transposed,
 // at `dst_t` straight from the registers, where a lane holds four consecutive rows of one column.  Either may be NULL.
-__device__ inline void ns_store(const f32x16& v, unsigned* patch, char* dst, long pitch, char* dst_t, long pitch_t) {
+__device__ inline void ns_store(const f32x16& v, unsigned* patch, gbytes dst, gbytes dst_t) {
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
     unsigned u[16];
 #pragma unroll
@@ -330,10 +372,10 @@ __device__ inline void ns_store(const f32x16& v, unsigned* patch, char* dst, lon
     if (dst_t) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            char* p = dst_t + col * pitch_t + (8 * q + 4 * half) * 2;
+            gbytes p = dst_t + col * 128 + (8 * q + 4 * half) * 2;
             const unsigned* w = u + 4 * q;
-            *reinterpret_cast<u32x2*>(p) = u32x2{(w[0] & 0xffffu) | (w[1] << 16), (w[2] & 0xffffu) | (w[3] << 16)};
-            *reinterpret_cast<u32x2*>(p + 64) = u32x2{(w[0] >> 16) | (w[1] & 0xffff0000u), (w[2] >> 16) | (w[3] & 0xffff0000u)};
+            *(DVAE_GLOBAL u32x2*)(p) = u32x2{(w[0] & 0xffffu) | (w[1] << 16), (w[2] & 0xffffu) | (w[3] << 16)};
+            *(DVAE_GLOBAL u32x2*)(p + 64) = u32x2{(w[0] >> 16) | (w[1] & 0xffff0000u), (w[2] >> 16) | (w[3] & 0xffff0000u)};
         }
     }
     if (dst) {
@@ -347,10 +389,10 @@ __device__ inline void ns_store(const f32x16& v, unsigned* patch, char* dst, lon
         for (int k = 0; k < 2; ++k) {
             const int r = (lane >> 2) + 16 * k, c = (lane & 3) * 8;
             const u32x4 a = *reinterpret_cast<const u32x4*>(patch + r * ST + c), b = *reinterpret_cast<const u32x4*>(patch + r * ST + c + 4);
-            char* p = dst + r * pitch + c * 2;
-            *reinterpret_cast<u32x4*>(p) = u32x4{(a[0] & 0xffffu) | (a[1] << 16), (a[2] & 0xffffu) | (a[3] << 16),
+            gbytes p = dst + r * 128 + c * 2;
+            *(DVAE_GLOBAL u32x4*)(p) = u32x4{(a[0] & 0xffffu) | (a[1] << 16), (a[2] & 0xffffu) | (a[3] << 16),
                                                  (b[0] & 0xffffu) | (b[1] << 16), (b[2] & 0xffffu) | (b[3] << 16)};
-            *reinterpret_cast<u32x4*>(p + 64) = u32x4{(a[0] >> 16) | (a[1] & 0xffff0000u), (a[2] >> 16) | (a[3] & 0xffff0000u),
+            *(DVAE_GLOBAL u32x4*)(p + 64) = u32x4{(a[0] >> 16) | (a[1] & 0xffff0000u), (a[2] >> 16) | (a[3] & 0xffff0000u),
                                                       (b[0] >> 16) | (b[1] & 0xffff0000u), (b[2] >> 16) | (b[3] & 0xffff0000u)};
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -369,19 +411,17 @@ __device__ inline void ns_triangle(int t, int& i, int& k) {
 // The symmetric products store the tiles at and below the diagonal and their mirror images.  Tiles on the diagonal are
 // stored once: their two halves agree to rounding only, and two writers of one place would leave either's.
 template <int TS>
-__device__ inline void ns_store_symmetric(NsTile<TS>& c, char* smem, char* dst, int P, int ti, int tk) {
+__device__ inline void ns_store_symmetric(NsTile<TS>& c, char* smem, gbytes dst, int P, int ti, int tk) {
     constexpr int S = NsTile<TS>::S;
     const int wave = threadIdx.x >> 6, wr = (wave >> 1) * (TS / 2), wc = (wave & 1) * (TS / 2);
     unsigned* patch = reinterpret_cast<unsigned*>(smem) + wave * (32 * 36);
-    const long pitch = 4L * P;
 #pragma unroll
     for (int i = 0; i < S; ++i)
 #pragma unroll
         for (int k = 0; k < S; ++k) {
             const int row = ti * TS + wr + i * 32, col = tk * TS + wc + k * 32;
             if (row >= P || col >= P) continue;
-            ns_store(c.acc[i][k], patch, dst + row * pitch + (col >> 5) * 128L, pitch,
-                     ti != tk ? dst + col * pitch + (row >> 5) * 128L : nullptr, pitch);
+            ns_store(c.acc[i][k], patch, ns_line(dst, P, row, col), ti != tk ? ns_line(dst, P, col, row) : gbytes(nullptr));
         }
 }
 
@@ -401,7 +441,7 @@ __global__ __launch_bounds__(256, 2) void ns_gram_kernel(NsArgs g) {
     const int line0 = PIECES ? t % pieces * g.kc : 0;
     NsTile<TS> c;
     c.zero();
-    c.run(w.x, 4L * w.Q, ti * TS, w.P, w.x, 4L * w.Q, tk * TS, w.P, line0, PIECES ? min(g.kc, lines - line0) : lines, smem);
+    c.run(w.x, w.P, ti * TS, w.x, w.P, tk * TS, line0, PIECES ? min(g.kc, lines - line0) : lines, smem);
     if (PIECES) {
         float* out = g.part + (long)wg * (TS * TS) + threadIdx.x;
 #pragma unroll
@@ -433,13 +473,18 @@ __global__ __launch_bounds__(256) void ns_gram_sum_kernel(NsArgs g) {
     const float* in = g.part + ((long)g.first[NS_GRAM * g.jp + jn] + (long)t * pieces) * (TS * TS) + threadIdx.x;
     NsTile<TS> c;
     c.zero();
-    for (int s = 0; s < pieces; ++s, in += TS * TS)
+    static_assert(S == 1, "pieces are cut for tiles of 64");
+    for (int s = 0; s < pieces; s += 4, in += 4 * TS * TS) {          // four pieces' loads in flight
+        float v[4][16];
 #pragma unroll
-        for (int i = 0; i < S; ++i)
+        for (int u = 0; u < 4; ++u)
 #pragma unroll
-            for (int k = 0; k < S; ++k)
+            for (int e = 0; e < 16; ++e) v[u][e] = s + u < pieces ? in[u * TS * TS + e * 256] : 0.f;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) c.acc[i][k][e] += in[((i * S + k) * 16 + e) * 256];
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) c.acc[0][0][e] += v[u][e];
+    }
 #pragma unroll
     for (int i = 0; i < S; ++i)
 #pragma unroll
@@ -462,8 +507,7 @@ __global__ __launch_bounds__(256, 2) void ns_square_kernel(NsArgs g) {
     ns_triangle(t, ti, tk);
     NsTile<TS> c;
     c.zero();
-    const long pitch = 4L * w.P;
-    c.run(w.a, pitch, ti * TS, w.P, w.a, pitch, tk * TS, w.P, 0, w.P / 32, smem);
+    c.run(w.a, w.P, ti * TS, w.a, w.P, tk * TS, 0, w.P / 32, smem);
     const float s2 = g.c * (NS_SB / (NS_SA * NS_SA)), s1 = g.b * (NS_SB / NS_SA), s0 = g.a * NS_SB;
 #pragma unroll
     for (int i = 0; i < S; ++i)
@@ -472,10 +516,10 @@ __global__ __launch_bounds__(256, 2) void ns_square_kernel(NsArgs g) {
             const int col = tk * TS + NsTile<TS>::col_of(k), row = ti * TS + NsTile<TS>::row_of(i, 0);
             if (col >= w.P || row >= w.P) continue;
             // a lane's elements of A lie along a column: read as a row, A being symmetric
-            const char* p = w.a + col * pitch + (row >> 5) * 128L + (row & 31) * 2;
+            cgbytes p = ns_line(w.a, w.P, col, row & ~31) + (row & 31) * 2;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const u32x2 h = *reinterpret_cast<const u32x2*>(p + 16 * q), l = *reinterpret_cast<const u32x2*>(p + 16 * q + 64);
+                const u32x2 h = *(const DVAE_GLOBAL u32x2*)(p + 16 * q), l = *(const DVAE_GLOBAL u32x2*)(p + 16 * q + 64);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const f16x2 hv = __builtin_bit_cast(f16x2, (unsigned)h[e >> 1]), lv = __builtin_bit_cast(f16x2, (unsigned)l[e >> 1]);
@@ -500,8 +544,7 @@ __global__ __launch_bounds__(256, 2) void ns_apply_kernel(NsArgs g) {
     const int ni = (w.P + TS - 1) / TS, ti = t % ni, tk = t / ni;
     NsTile<TS> c;
     c.zero();
-    const long pp = 4L * w.P, pq = 4L * w.Q;
-    c.run(w.b, pp, ti * TS, w.P, w.xt[g.turn], pp, tk * TS, w.Q, 0, w.P / 32, smem);
+    c.run(w.b, w.P, ti * TS, w.xt(g.turn), w.Q, tk * TS, 0, w.P / 32, smem);
     const int wave = threadIdx.x >> 6, wr = (wave >> 1) * (TS / 2), wc = (wave & 1) * (TS / 2);
     unsigned* patch = reinterpret_cast<unsigned*>(smem) + wave * (32 * 36);
 #pragma unroll
@@ -512,7 +555,7 @@ __global__ __launch_bounds__(256, 2) void ns_apply_kernel(NsArgs g) {
             if (row >= w.P || col >= w.Q) continue;
 #pragma unroll
             for (int e = 0; e < 16; ++e) c.acc[i][k][e] *= 1.f / NS_SB;
-            ns_store(c.acc[i][k], patch, w.x + row * pq + (col >> 5) * 128L, pq, w.xt[g.turn ^ 1] + col * pp + (row >> 5) * 128L, pp);
+            ns_store(c.acc[i][k], patch, ns_line(w.x, w.P, row, col), ns_line(w.xt(g.turn ^ 1), w.Q, col, row));
         }
 }
 
@@ -529,11 +572,10 @@ __global__ __launch_bounds__(256, 2) void ns_last_kernel(NsArgs g) {
     const int ni = (w.P + TS - 1) / TS, tp = t % ni, tq = t / ni;
     NsTile<TS> c;
     c.zero();
-    const long pp = 4L * w.P;
-    const char *L = tall ? w.xt[g.turn] : w.b, *R = tall ? w.b : w.xt[g.turn];
+    const cgbytes L = tall ? w.xt(g.turn) : w.b, R = tall ? w.b : w.xt(g.turn);
     const int lrows = tall ? w.Q : w.P, rrows = tall ? w.P : w.Q, ti = tall ? tq : tp, tk = tall ? tp : tq;
-    c.run(L, pp, ti * TS, lrows, R, pp, tk * TS, rrows, 0, w.P / 32, smem);
-    T* out = (T*)j.out;
+    c.run(L, lrows, ti * TS, R, rrows, tk * TS, 0, w.P / 32, smem);
+    const auto out = as_global<T>(j.out);
     const float step = MUON ? g.lr * j.scale : 0.f;
 #pragma unroll
     for (int i = 0; i < S; ++i)

@@ -1,0 +1,365 @@
+// The whole iteration of a small matrix (p <= 64, q <= 768) in one workgroup and one launch: momentum, norm, every step, the
+// result or the parameter's update.  What bounds such matrices is not work (64 x 576: 0.3 GFLOP of MFMAs) but the chain of
+// dependent launches, four a step through the batched kernels, about 5 us each.
+//
+// Eight waves; wave w owns the 32-column blocks w, w + 8, .. of X (NB at most) and keeps them in registers for good, as
+// MFMA fragments: a product's accumulator X^T[q][p] has p across lanes and q down the registers, which is an operand of
+// X X^T as it stands (contraction over q, in whatever order both operands share).  Per step:
+//   Gram     every wave its blocks, 3 of the 4 subtiles of A (p x p), partial sums through LDS
+//   square   A in LDS as plane pairs, B = a I + b A + c A^2, two of its sixteen subtiles a wave, back to LDS
+//   apply    X^T <- X^T B, block by block: the one transposition (lanes to q) goes through a patch of LDS of the wave's own
+// Three barriers a step.  Numbers are held as in the batched kernels: two fp16 pieces, three MFMAs, fp32 sums.
+#pragma once
+#include "newton_schulz.hpp"
+
+namespace dvae {
+
+using f16x4 = __attribute__((ext_vector_type(4))) _Float16;
+
+constexpr int NS_SMALL_P = 64, NS_SMALL_Q = 768, NS_SMALL_VEC = 1 << 15, NS_SMALL_JOBS = 32;
+
+struct NsSmallArgs {
+    NsJob jobs[NS_SMALL_JOBS];
+    double eps;
+    float a, b, c;
+    float mu, nu, lr, decay;
+    int nesterov, steps;
+};
+static_assert(sizeof(NsSmallArgs) <= 4096, "kernel arguments");
+
+struct NsSmallLds {
+    // A wave's partial Gram subtiles, four rows of a lane's column at a time: [3][4][lane][4].  Between two Grams the wave's
+    // transposition patch lies in them: [32 q] rows of 64 h's and 64 l's of p, PITCH bytes apart (16-byte reads of 16 rows meet
+    // all banks once), or of 64 floats while the matrix comes and goes.
+    static constexpr int PITCH = 272;
+    f32x4 sum[8][3 * 4 * 64];
+    char a[64 * 256], b[64 * 256];                        // plane pairs, [line][row], chunks swizzled as in NsTile
+    double red[8];
+};
+
+// 16-byte chunk `chunk` of row `row` of line `line`
+__device__ inline int ns_small_at(int line, int row, int chunk) { return (line * 64 + row) * 128 + ((chunk ^ (row >> 1 & 7)) << 4); }
+
+// what lanes of a wave wrote to LDS is there for its other lanes
+__device__ inline void ns_wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+struct NsBlock {
+    f16x8 h[2][2], l[2][2];                               // [32 rows of p][half of the block's q]
+};
+
+template <typename T, bool MUON, int NB>
+__global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
+    extern __shared__ __align__(16) char smem[];
+    NsSmallLds& s = *reinterpret_cast<NsSmallLds*>(smem);
+    const NsJob& j = g.jobs[blockIdx.x];
+    const int m = j.m, n = j.n;
+    const long xs = j.xs, os = j.os;
+    const auto x = as_global<const T>(j.x);
+    const auto out = as_global<T>(j.out);
+    const auto mom = as_global<float>(j.mom);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
+    if (MUON && j.vec) {
+        for (long e = threadIdx.x; e < n; e += 512) {
+            const float gr = (float)x[e], p = (float)out[e];
+            const float mi = g.mu * mom[e] + g.nu * gr;
+            mom[e] = mi;
+            out[e] = (T)(p * g.decay - g.lr * (g.nesterov ? g.nu * gr + g.mu * mi : mi));
+        }
+        return;
+    }
+    const bool tall = m > n;
+    const int p = tall ? n : m, q = tall ? m : n;
+    constexpr int PITCH = NsSmallLds::PITCH / 4;
+    float* patch = reinterpret_cast<float*>(s.sum[wave]);
+
+    // A block's elements as the caller's memory has them along lanes: a tall matrix's rows hold p (one q at a time), another's
+    // q (32 of two p's).  Element i of half t is (qi, pi) of the block, at start + i * leap.
+    auto qi_of = [&](int t, int i) { return tall ? t * 16 + i : col; };
+    auto pi_of = [&](int t, int i) { return tall ? lane : (t * 16 + i) * 2 + half; };
+    auto start_of = [&](int q0, int t, long stride) {
+        return tall ? (long)(q0 + t * 16) * stride + lane : (long)(t * 32 + half) * stride + q0 + col;
+    };
+
+    // ---- load, all of it in flight at once; then u and its norm, and through the patch to [q][p] ---------------------
+    float raw[NB][2][16];
+    double sq = 0.0;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+        const int q0 = (wave + 8 * k) * 32;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const long start = start_of(q0, t, xs), leap = tall ? xs : 2 * xs;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)                  // elements past the edge read the first one and count as zero
+                raw[k][t][i] = (float)x[q0 + qi_of(t, i) < q && pi_of(t, i) < p ? start + i * leap : 0L];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+        const int q0 = (wave + 8 * k) * 32;
+        if (q0 < q) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const long start = start_of(q0, t, xs), leap = tall ? xs : 2 * xs;
+                float mv[16];
+                if (MUON) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) mv[i] = mom[q0 + qi_of(t, i) < q && pi_of(t, i) < p ? start + i * leap : 0L];
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const bool in = q0 + qi_of(t, i) < q && pi_of(t, i) < p;
+                    float v = in ? raw[k][t][i] : 0.f;
+                    if (MUON) {
+                        const float mi = in ? g.mu * mv[i] + g.nu * v : 0.f;
+                        if (in) mom[start + i * leap] = mi;
+                        v = g.nesterov ? g.nu * v + g.mu * mi : mi;
+                    }
+                    sq += (double)v * (double)v;
+                    patch[qi_of(t, i) * PITCH + pi_of(t, i)] = v;
+                }
+            }
+            ns_wave_sync();
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float v = patch[(8 * (e >> 2) + 4 * half + (e & 3)) * PITCH + i * 32 + col];
+                raw[k][i][e] = q0 < q ? v : 0.f;
+            }
+        ns_wave_sync();
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sq += __shfl_xor(sq, o, 64);
+    if (lane == 0) s.red[wave] = sq;
+    __syncthreads();
+    sq = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sq += s.red[i];
+    // times 2^14 / (norm + eps), as a power of two and a factor near one: a float does not hold it for every norm
+    int shift;
+    const float factor = (float)frexp((double)NS_SX / (sqrt(sq) + g.eps), &shift);
+
+    NsBlock blk[NB];
+    // v times `by`, a power of two (so that the product is exact, see ns_rounded), in two pieces; element e of a subtile, e = 8 t + i, is element i of the fragment of half t
+    auto hold = [&](NsBlock& b, int i, const float (&v)[16], float by) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const f16 h = (f16)(v[8 * t + e] * by);
+                b.h[i][t][e] = h;
+                b.l[i][t][e] = (f16)__builtin_fmaf(v[8 * t + e], by, -(float)h);
+            }
+    };
+#pragma unroll
+    for (int k = 0; k < NB; ++k)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float v[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = ns_rounded(ldexpf(raw[k][i][e], shift) * factor);
+            hold(blk[k], i, v, 1.f);
+        }
+
+    const int used = min(8, (q + 31) / 32);               // waves that own a block
+    for (int step = 0; step < g.steps; ++step) {
+        // Addresses are worked out anew in every step: the compiler would hold some hundred of them over the loop, in registers
+        // that the matrix needs.
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));
+        const int col = lane & 31, half = lane >> 5;
+        // ---- Gram ----
+        if (wave < used) {
+            f32x16 acc[3];
+#pragma unroll
+            for (int t = 0; t < 3; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[t][e] = 0.f;
+#pragma unroll
+            for (int k = 0; k < NB; ++k) {
+                const NsBlock& b = blk[k];                // a block past q holds zeros
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    // subtiles (0,0), (1,0), (1,1)
+                    acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b.h[0][t], b.l[0][t], acc[0], 0, 0, 0);
+                    acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b.h[1][t], b.l[0][t], acc[1], 0, 0, 0);
+                    acc[2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b.h[1][t], b.l[1][t], acc[2], 0, 0, 0);
+                    acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b.l[0][t], b.h[0][t], acc[0], 0, 0, 0);
+                    acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b.l[1][t], b.h[0][t], acc[1], 0, 0, 0);
+                    acc[2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b.l[1][t], b.h[1][t], acc[2], 0, 0, 0);
+                    acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b.h[0][t], b.h[0][t], acc[0], 0, 0, 0);
+                    acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b.h[1][t], b.h[0][t], acc[1], 0, 0, 0);
+                    acc[2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b.h[1][t], b.h[1][t], acc[2], 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 3; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    s.sum[wave][(t * 4 + e) * 64 + lane] = f32x4{acc[t][4 * e], acc[t][4 * e + 1], acc[t][4 * e + 2], acc[t][4 * e + 3]};
+        }
+        __syncthreads();
+        // ---- A: twelve groups of four rows of a subtile, to waves 0 .. 7 and 0 .. 3 ----
+        for (int task = wave; task < 12; task += 8) {
+            f32x4 part[8];
+#pragma unroll
+            for (int w = 0; w < 8; ++w) {
+                part[w] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (w < used) part[w] = s.sum[w][task * 64 + lane];
+            }
+            const f32x4 v = ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
+            const int t = task >> 2;
+            const int row = (t ? 32 : 0) + 8 * (task & 3) + 4 * half, c = (t == 2 ? 32 : 0) + col;
+            f16x4 h, l;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float f = ns_rounded(v[i] * (NS_SA / (NS_SX * NS_SX)));
+                h[i] = (f16)f;
+                l[i] = (f16)(f - (float)h[i]);
+            }
+            // the lane's four rows of column c are four columns of row c; the subtile below the diagonal is stored as it is, too
+            const int chunk = (row & 31) >> 3;
+            *reinterpret_cast<f16x4*>(s.a + ns_small_at(row >> 5, c, chunk) + (row & 7) * 2) = h;
+            *reinterpret_cast<f16x4*>(s.a + ns_small_at(row >> 5, c, 4 + chunk) + (row & 7) * 2) = l;
+            if (t == 1) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    *reinterpret_cast<f16*>(s.a + ns_small_at(0, row + i, c >> 3) + (c & 7) * 2) = h[i];
+                    *reinterpret_cast<f16*>(s.a + ns_small_at(0, row + i, 4 + (c >> 3)) + (c & 7) * 2) = l[i];
+                }
+            }
+        }
+        __syncthreads();
+        // ---- square: two 16x16 subtiles a wave, their lines a 16x16x32 MFMA each ----
+        {
+            const int r16 = lane & 15, quarter = lane >> 4;
+            const float s2 = g.c * (NS_SB / (NS_SA * NS_SA)), s1 = g.b * (NS_SB / NS_SA), s0 = g.a * NS_SB;
+            const int ti = wave >> 1;
+            f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int line = 0; line < 2; ++line) {
+                const f16x8 lh = *reinterpret_cast<const f16x8*>(s.a + ns_small_at(line, ti * 16 + r16, quarter));
+                const f16x8 ll = *reinterpret_cast<const f16x8*>(s.a + ns_small_at(line, ti * 16 + r16, 4 + quarter));
+                f16x8 rh[2], rl[2];
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const int row = ((wave & 1) * 2 + n) * 16 + r16;
+                    rh[n] = *reinterpret_cast<const f16x8*>(s.a + ns_small_at(line, row, quarter));
+                    rl[n] = *reinterpret_cast<const f16x8*>(s.a + ns_small_at(line, row, 4 + quarter));
+                }
+#pragma unroll
+                for (int n = 0; n < 2; ++n) acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lh, rl[n], acc[n], 0, 0, 0);
+#pragma unroll
+                for (int n = 0; n < 2; ++n) acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ll, rh[n], acc[n], 0, 0, 0);
+#pragma unroll
+                for (int n = 0; n < 2; ++n) acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lh, rh[n], acc[n], 0, 0, 0);
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                // rows r0 .. r0 + 3 of column c, that is of row c, A being symmetric
+                const int c = ((wave & 1) * 2 + n) * 16 + r16, r0 = ti * 16 + 4 * quarter;
+                const int ah = ns_small_at(r0 >> 5, c, (r0 & 31) >> 3) + (r0 & 7) * 2, al = ns_small_at(r0 >> 5, c, 4 + ((r0 & 31) >> 3)) + (r0 & 7) * 2;
+                const f16x4 vh = *reinterpret_cast<const f16x4*>(s.a + ah), vl = *reinterpret_cast<const f16x4*>(s.a + al);
+                f16x4 h, l;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float r = s2 * acc[n][i] + s1 * ((float)vh[i] + (float)vl[i]);
+                    if (r0 + i == c) r += s0;
+                    r = ns_rounded(r);
+                    h[i] = (f16)r;
+                    l[i] = (f16)(r - (float)h[i]);
+                }
+                *reinterpret_cast<f16x4*>(s.b + ah) = h;
+                *reinterpret_cast<f16x4*>(s.b + al) = l;
+            }
+        }
+        __syncthreads();
+        // ---- apply ----
+        char* xt = reinterpret_cast<char*>(s.sum[wave]);
+#pragma unroll
+        for (int k = 0; k < NB; ++k) {
+            const int q0 = (wave + 8 * k) * 32;
+            if (q0 < q) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        char* at = xt + (8 * (e >> 2) + 4 * half + (e & 3)) * NsSmallLds::PITCH + (i * 32 + col) * 2;
+                        *reinterpret_cast<f16*>(at) = blk[k].h[i][e >> 3][e & 7];
+                        *reinterpret_cast<f16*>(at + 128) = blk[k].l[i][e >> 3][e & 7];
+                    }
+                ns_wave_sync();
+                f32x16 acc[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) {
+                    const int line = kk >> 1, t = kk & 1;
+                    const f16x8 lh = *reinterpret_cast<const f16x8*>(xt + col * NsSmallLds::PITCH + kk * 32 + half * 16);
+                    const f16x8 ll = *reinterpret_cast<const f16x8*>(xt + col * NsSmallLds::PITCH + 128 + kk * 32 + half * 16);
+                    f16x8 rh[2], rl[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        rh[i] = *reinterpret_cast<const f16x8*>(s.b + ns_small_at(line, i * 32 + col, t * 2 + half));
+                        rl[i] = *reinterpret_cast<const f16x8*>(s.b + ns_small_at(line, i * 32 + col, 4 + t * 2 + half));
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh, rl[i], acc[i], 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ll, rh[i], acc[i], 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh, rh[i], acc[i], 0, 0, 0);
+                }
+                ns_wave_sync();
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float v[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) v[e] = acc[i][e];
+                    hold(blk[k], i, v, 1.f / NS_SB);
+                }
+            }
+        }
+    }
+
+    // ---- the result: back through the patch, so that lanes run along the caller's rows -------------------------------
+    const float step_len = MUON ? g.lr * j.scale : 0.f;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+        const int q0 = (wave + 8 * k) * 32;
+        if (q0 < q) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    patch[(8 * (e >> 2) + 4 * half + (e & 3)) * PITCH + i * 32 + col] =
+                        ((float)blk[k].h[i][e >> 3][e & 7] + (float)blk[k].l[i][e >> 3][e & 7]) * (1.f / NS_SX);
+            ns_wave_sync();
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const long start = start_of(q0, t, os), leap = tall ? os : 2 * os;
+                float old[16];
+                if (MUON) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) old[i] = (float)out[q0 + qi_of(t, i) < q && pi_of(t, i) < p ? start + i * leap : 0L];
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float v = patch[qi_of(t, i) * PITCH + pi_of(t, i)];
+                    if (q0 + qi_of(t, i) < q && pi_of(t, i) < p) out[start + i * leap] = (T)(MUON ? old[i] * g.decay - step_len * v : v);
+                }
+            }
+            ns_wave_sync();
+        }
+    }
+}
+
+}  // namespace dvae

@@ -28,7 +28,8 @@ def held(got, x, **kw):
 
 
 SHAPES = [(1, 1), (1, 2), (5, 1), (2, 2), (3, 288), (10, 2100), (27, 64), (64, 27), (31, 33), (63, 64), (64, 64), (64, 65), (65, 64),
-          (64, 576), (576, 64), (96, 96), (127, 129), (128, 128), (129, 127), (128, 1152), (200, 130), (256, 300), (320, 700)]
+          (64, 576), (576, 64), (96, 96), (127, 129), (128, 128), (129, 127), (128, 1152), (200, 130), (256, 300), (320, 700),
+          (33, 512), (50, 257), (257, 20), (64, 768), (767, 63), (64, 769), (65, 768)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -169,7 +170,9 @@ def test_step(kw):
 
 
 def test_many_parameters():
-    step_held([(24, 5 + i % 40) if i % 3 else (i + 1,) for i in range(150)], seed=4)
+    step_held([(24, 5 + i % 40) if i % 3 else (i + 1,) for i in range(150)], seed=4)       # one launch for every 32 of them
+    step_held([(24, 5 + i % 40) if i % 3 else (i + 1,) for i in range(149)] + [(70, 70)], seed=5)     # the batched phases
+    step_held([(40, 3, 3, 3), (40000,), (9,)], seed=6)
 
 
 def test_vectors_only_and_views_of_a_bucket():

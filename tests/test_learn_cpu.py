@@ -52,7 +52,7 @@ def test_newton_schulz_and_muon_refuse_bad_arguments():
                 dict(ws=F + 64), dict(count=-1), dict(coef=(9.0, 0, 0)), dict(coef=(3.0, 0, 0)), dict(coef=(1.0, 5.0, 0)),
                 dict(coef=(float("nan"), 0, 0))):
         assert call(**bad) == -1 and b"newton_schulz" in lib.dvae_last_error(), bad
-    assert call(n=1024) == -4 and call(dt=3) == -2
+    assert call(n=100) == -4 and call(dt=3) == -2 and call(row=(F, F, F, 65, 65, 65, 65, 0), n=1024) == -4
 
     def muon(row=good, lr=0.1, mu=0.9, wd=0.0, rule=0, n=1 << 40):
         t, c = table(row), array("d", COEF)
