@@ -4,6 +4,7 @@
 #include <limits.h>
 #include <math.h>
 
+#include <algorithm>
 #include <vector>
 
 #include "common.hpp"
@@ -132,10 +133,10 @@ inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 struct NsPlan {
     std::vector<unsigned> table;      // prefix arrays, then jobs, as they lie on the device
     int njobs = 0, jp = 0;
-    long total[NS_PHASES] = {0, 0, 0, 0, 0};
-    int gram_ts = 64, sym_ts = 64, apply_ts = 64;
-    bool pieces = false;
-    int kc = 0;
+    long total[NS_PHASES] = {};
+    int gram_ts = 64, square_ts = 64, apply_ts = 64;
+    int apply_groups = 1;
+    bool gram_pieces = false;
     size_t norm_off = 0, part_off = 0, bytes = 0;
     bool matrices = false;
 };
@@ -248,33 +249,59 @@ int ns_plan(const char* what, const dvae_matrix* mats, int count, int scale_rule
     p.jp = (count + 1 + 63) / 64 * 64;
     std::vector<NsJob> jobs((size_t)count);
     std::vector<int> first((size_t)NS_PHASES * p.jp, INT_MAX);
-    // Tiles of 128 read half as much LDS per product as tiles of 64, and want enough of them: the larger tile is taken
-    // where its tiles alone give every CU one.
-    long big_apply = 0, big_sym = 0, sym64 = 0, lines64 = 0, longest = 0;
+    // Tile sizes by the work they make, in us of a CU: a line of a 128-tile costs it 0.78, of a 64-tile 0.28 (measured with the chip
+    // full; a 128-tile is four of those), and a tile's start and end about 3 and 1.2.  Padding decides: 64-row matrices want 64.
+    double cost[3][2] = {};                               // Gram, square, apply; tiles of 64, of 128
+    long longest[2] = {1, 1}, lines[2] = {}, tiles[3][2] = {}, tiles32 = 0;
     for (int i = 0; i < count; ++i) {
         const dvae_matrix& m = mats[i];
         if (m.vector) continue;
-        const long P = ns_pad((int)(m.rows < m.cols ? m.rows : m.cols)), Q = ns_pad((int)(m.rows < m.cols ? m.cols : m.rows));
-        big_apply += (P + 127) / 128 * ((Q + 127) / 128);
-        big_sym += ns_triangles((int)P, 128);
-        sym64 += ns_triangles((int)P, 64);
-        lines64 += ns_triangles((int)P, 64) * (Q / 32);
-        longest = longest > Q / 32 ? longest : Q / 32;
+        const int P = ns_pad((int)(m.rows < m.cols ? m.rows : m.cols)), Q = ns_pad((int)(m.rows < m.cols ? m.cols : m.rows));
+        for (int big = 0; big < 2; ++big) {
+            const int ts = big ? 128 : 64;
+            const double line = big ? 0.78 : 0.28, ends = big ? 3.0 : 1.2;
+            const long tri = ns_triangles(P, ts);
+            cost[0][big] += tri * (Q / 32 * line + ends);
+            cost[1][big] += tri * (P / 32 * line + ends);
+            cost[2][big] += (double)((P + ts - 1) / ts) * ((Q + ts - 1) / ts) * (P / 32 * line + ends);
+            lines[big] += tri * (Q / 32);
+            tiles[0][big] += tri;
+            tiles[1][big] += tri;
+            tiles[2][big] += (long)((P + ts - 1) / ts) * ((Q + ts - 1) / ts);
+        }
+        tiles32 += ns_triangles(P, 32);
+        longest[0] = longest[0] > Q / 32 ? longest[0] : Q / 32;
+        longest[1] = longest[1] > P / 32 ? longest[1] : P / 32;
         p.matrices = true;
     }
-    p.apply_ts = big_apply >= 256 ? 128 : 64;
-    p.sym_ts = big_sym >= 256 ? 128 : 64;
-    p.gram_ts = p.sym_ts;
-    // The Gram phase has few tiles and a long contraction: below 512 workgroups it is cut into pieces of equal length.
-    if (p.gram_ts == 64 && sym64 < 512) {
-        p.kc = (int)((lines64 + 511) / 512);
-        if (p.kc < 4) p.kc = 4;
-        if (p.kc < (longest + 31) / 32) p.kc = (int)((longest + 31) / 32);      // at most 32 of a tile, which one workgroup adds up
-        p.kc = (p.kc + 1) & ~1;
-    }
+    p.gram_ts = cost[0][1] < cost[0][0] ? 128 : 64;
+    // a product of one tile a workgroup: 128 only where that still gives every CU one
+    p.apply_ts = cost[2][1] < cost[2][0] && cost[2][1] / 256 >= 0.9 * (longest[1] * 0.78 + 3.0) ? 128 : 64;
+    // The Gram product in pieces: about 512 workgroups, two a CU, of at least 4 lines; none where tiles of 64 alone are as many
+    // (2048 x 2048: 53 us whole in tiles of 64, 45 + 12 us in pieces of tiles of 128).
+    const bool cut_gram = tiles[0][0] < 512;
+    if (!cut_gram && tiles[0][1] < 512) p.gram_ts = 64;
+    const int gb = p.gram_ts == 128;
+    const int gram_kc = (int)((lines[gb] + 511) / 512);
+    // The square has p / 32 lines and few tiles: straight from memory in tiles of 32 up to about two workgroups of those a SIMD
+    // (beyond, they read more than the L2 gives), whole in tiles of 64 until those of 128 fill the chip.
+    p.square_ts = tiles32 <= 1280 ? 32 : tiles[1][1] >= 512 ? 128 : 64;
+    // Two groups, see NsTile, where tiles of 128 are no more than the CUs (2048 x 2048: 68 -> 64 us).
+    p.apply_groups = p.apply_ts == 128 && tiles[2][1] <= 256 ? 2 : 1;
+    auto piece = [](bool cut, int kc, int all) {          // at most 64 of a tile; even
+        if (!cut) return all;
+        if (kc < 4) kc = 4;
+        if (kc < (all + 63) / 64) kc = (all + 63) / 64;
+        return (kc + 1) & ~1;
+    };
     long off = 0, part = 0;
+    // The matrices with the longest contractions go first, so that no long tile starts when the short ones are done.
+    std::vector<int> order((size_t)count);
+    for (int i = 0; i < count; ++i) order[i] = i;
+    auto side = [&](int i) { return mats[i].vector ? 0 : mats[i].rows < mats[i].cols ? mats[i].rows : mats[i].cols; };
+    std::stable_sort(order.begin(), order.end(), [&](int a, int b) { return side(a) > side(b); });
     for (int i = 0; i < count; ++i) {
-        const dvae_matrix& m = mats[i];
+        const dvae_matrix& m = mats[order[i]];
         NsJob& j = jobs[i];
         ns_job(m, scale_rule, j);
         const long chunks = ((long)j.m * j.n + NS_CHUNK - 1) / NS_CHUNK;
@@ -291,10 +318,12 @@ int ns_plan(const char* what, const dvae_matrix* mats, int count, int scale_rule
         const int P = ns_pad(j.m < j.n ? j.m : j.n), Q = ns_pad(j.m < j.n ? j.n : j.m);
         off += ns_job_bytes(j.m, j.n);
         p.total[NS_SPLIT] += (long)(P / 64) * (Q / 64);
-        const long pieces = p.kc ? (Q / 32 + p.kc - 1) / p.kc : 1;
-        if (pieces > 1) p.pieces = true;
-        p.total[NS_GRAM] += ns_triangles(P, p.gram_ts) * pieces;
-        p.total[NS_SYM] += ns_triangles(P, p.sym_ts);
+        j.kc = piece(cut_gram, gram_kc, Q / 32);
+        const long gp = (Q / 32 + j.kc - 1) / j.kc;
+        if (gp > 1) p.gram_pieces = true;
+        p.total[NS_GRAM] += ns_triangles(P, p.gram_ts) * gp;
+        p.total[NS_GRAM_TILES] += ns_triangles(P, p.gram_ts);
+        p.total[NS_SQUARE] += ns_triangles(P, p.square_ts);
         p.total[NS_APPLY] += (long)((P + p.apply_ts - 1) / p.apply_ts) * ((Q + p.apply_ts - 1) / p.apply_ts);
     }
     for (int f = 0; f < NS_PHASES; ++f)
@@ -306,7 +335,9 @@ int ns_plan(const char* what, const dvae_matrix* mats, int count, int scale_rule
     if (count) memcpy(p.table.data() + first.size(), jobs.data(), jobs.size() * sizeof(NsJob));
     p.norm_off = align256(words * 4);
     p.part_off = p.norm_off + align256((size_t)part * sizeof(double));
-    const size_t planes = p.part_off + (p.pieces ? align256((size_t)p.total[NS_GRAM] * 64 * 64 * 4) : 0);
+    size_t parts = 0;
+    if (p.gram_pieces) parts = (size_t)p.total[NS_GRAM] * p.gram_ts * p.gram_ts;
+    const size_t planes = p.part_off + align256(parts * 4);
     NsJob* t = reinterpret_cast<NsJob*>(p.table.data() + first.size());
     for (int i = 0; i < count; ++i) t[i].off += (long)planes;
     p.bytes = planes + (size_t)off;
@@ -317,7 +348,8 @@ template <typename T, bool MUON>
 int ns_run(const char* what, const NsPlan& p, NsArgs g, int steps, hipStream_t st) {
     // the table, as many kernel arguments at a time as fit
     NsBlob blob;
-    for (size_t at = 0; at < p.table.size(); at += NsBlob::WORDS) {
+    if (p.njobs == 1) memcpy(&g.one, p.table.data() + (size_t)NS_PHASES * p.jp, sizeof(NsJob));
+    else for (size_t at = 0; at < p.table.size(); at += NsBlob::WORDS) {
         const size_t n = p.table.size() - at < (size_t)NsBlob::WORDS ? p.table.size() - at : (size_t)NsBlob::WORDS;
         memcpy(blob.w, p.table.data() + at, n * 4);
         hipLaunchKernelGGL(ns_table_kernel, dim3(1), dim3(256), 0, st, blob, (unsigned*)g.ws + at, (int)n);
@@ -329,39 +361,53 @@ int ns_run(const char* what, const NsPlan& p, NsArgs g, int steps, hipStream_t s
     g.part = (float*)(g.ws + p.part_off);
     g.njobs = p.njobs;
     g.jp = p.jp;
-    g.kc = p.kc;
     g.turn = 0;
-#define NS_LAUNCH(kernel, phase)                                                                     \
+// n workgroups of 256 * groups threads with tiles of ts in LDS (0: none); kernels that want over 64 KB of it say so once
+#define NS_LAUNCH_N(n, groups, lds, ...)                                                             \
     do {                                                                                             \
-        g.total = (int)p.total[phase];                                                               \
-        hipLaunchKernelGGL((kernel), dim3((unsigned)p.total[phase]), dim3(256), 0, st, g);           \
+        static LdsOptIn opt;                                                                         \
+        if ((lds) > 65536) opt.ensure((const void*)(__VA_ARGS__), lds);                              \
+        g.total = (int)(n);                                                                          \
+        hipLaunchKernelGGL((__VA_ARGS__), dim3((unsigned)(n)), dim3(256 * (groups)), lds, st, g);    \
         DVAE_CHECK_LAUNCH(what);                                                                     \
     } while (0)
-    NS_LAUNCH((ns_norm_kernel<T, MUON>), NS_NORM);
+#define NS_LAUNCH(phase, ...) NS_LAUNCH_N(p.total[phase], 1, 0, __VA_ARGS__)
+#define NS_LAUNCH_TILES(phase, ts, groups, ...) NS_LAUNCH_N(p.total[phase], groups, (NsTile<ts, groups>::BYTES), __VA_ARGS__)
+    NS_LAUNCH(NS_NORM, ns_norm_kernel<T, MUON>);
     if (!p.matrices) return DVAE_OK;
-    NS_LAUNCH((ns_split_kernel<T, MUON>), NS_SPLIT);
+    NS_LAUNCH(NS_SPLIT, ns_split_kernel<T, MUON>);
     for (int k = 0; k < steps; ++k) {
-        if (p.pieces) {
-            NS_LAUNCH((ns_gram_kernel<64, true>), NS_GRAM);
-            NS_LAUNCH(ns_gram_sum_kernel<64>, NS_SYM);
-        } else if (p.gram_ts == 128) {
-            NS_LAUNCH((ns_gram_kernel<128, false>), NS_GRAM);
+        if (p.gram_ts == 64) {
+            if (!p.gram_pieces) NS_LAUNCH_TILES(NS_GRAM, 64, 1, ns_symmetric_kernel<64, false, false, 1>);
+            else {
+                NS_LAUNCH_TILES(NS_GRAM, 64, 1, ns_symmetric_kernel<64, false, true, 1>);
+                NS_LAUNCH_N(p.total[NS_GRAM_TILES] * 4, 1, 0, ns_gram_sum_kernel<64>);
+            }
+        } else if (!p.gram_pieces) {
+            NS_LAUNCH_TILES(NS_GRAM, 128, 1, ns_symmetric_kernel<128, false, false, 1>);
         } else {
-            NS_LAUNCH((ns_gram_kernel<64, false>), NS_GRAM);
+            NS_LAUNCH_TILES(NS_GRAM, 128, 1, ns_symmetric_kernel<128, false, true, 1>);
+            NS_LAUNCH_N(p.total[NS_GRAM_TILES] * 16, 1, 0, ns_gram_sum_kernel<128>);
         }
-        if (p.sym_ts == 128) NS_LAUNCH(ns_square_kernel<128>, NS_SYM);
-        else NS_LAUNCH(ns_square_kernel<64>, NS_SYM);
-        if (k + 1 < steps) {
-            if (p.apply_ts == 128) NS_LAUNCH(ns_apply_kernel<128>, NS_APPLY);
-            else NS_LAUNCH(ns_apply_kernel<64>, NS_APPLY);
-            g.turn ^= 1;
+        if (p.square_ts == 32) NS_LAUNCH(NS_SQUARE, ns_square_small_kernel);
+        else if (p.square_ts == 64) NS_LAUNCH_TILES(NS_SQUARE, 64, 1, ns_symmetric_kernel<64, true, false, 1>);
+        else NS_LAUNCH_TILES(NS_SQUARE, 128, 1, ns_symmetric_kernel<128, true, false, 1>);
+        const bool last = k + 1 == steps;
+        if (p.apply_ts == 128 && p.apply_groups == 1) {
+            if (last) NS_LAUNCH_TILES(NS_APPLY, 128, 1, ns_last_kernel<128, T, MUON, 1>);
+            else NS_LAUNCH_TILES(NS_APPLY, 128, 1, ns_apply_kernel<128, 1>);
         } else if (p.apply_ts == 128) {
-            NS_LAUNCH((ns_last_kernel<128, T, MUON>), NS_APPLY);
+            if (last) NS_LAUNCH_TILES(NS_APPLY, 128, 2, ns_last_kernel<128, T, MUON, 2>);
+            else NS_LAUNCH_TILES(NS_APPLY, 128, 2, ns_apply_kernel<128, 2>);
         } else {
-            NS_LAUNCH((ns_last_kernel<64, T, MUON>), NS_APPLY);
+            if (last) NS_LAUNCH_TILES(NS_APPLY, 64, 1, ns_last_kernel<64, T, MUON, 1>);
+            else NS_LAUNCH_TILES(NS_APPLY, 64, 1, ns_apply_kernel<64, 1>);
         }
+        g.turn ^= 1;
     }
+#undef NS_LAUNCH_TILES
 #undef NS_LAUNCH
+#undef NS_LAUNCH_N
     return DVAE_OK;
 }
 

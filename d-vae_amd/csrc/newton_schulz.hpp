@@ -11,10 +11,11 @@
 // hh + hl + lh, summed in fp32: the errors of an fp32 product at 3/16 of its time.  fp16's range is met by fixed scales: with
 // the coefficients' bounds checked on the host, |X| <= 2, |A| <= 4 and |B| <= 7, held as 2^14 X, 2^13 A and 2^13 B.
 //
-// Layout.  A plane pair of an R x K operand is made of lines of 128 bytes: 32 h's of a row, then the 32 l's of the same
-// columns.  The lines of the R rows follow each other, then those of the next 32 columns: what a tile reads or writes at a time
-// is one run of memory.  R and K are padded to 64 with zeros, which the products keep zero.  X is kept with its transpose (two copies,
-// taken in turn), so that every product reads both operands along its contraction and every store writes whole lines.
+// Layout.  An R x K operand is made of lines of 32 columns: a row's 32 h's, then its 32 l's, 128 bytes in eight chunks of 16.  Equal
+// chunks of the R rows follow each other, then the next chunk, then the next line: whatever a wave loads or stores, staged
+// tiles, fragments or either orientation of a result, is runs of 16 rows and more.  R and K are padded to 64 with zeros, which
+// the products keep zero.  X is kept with its transpose (two copies, taken in turn), so that every product reads both operands
+// along its contraction.
 #pragma once
 #include "common.hpp"
 
@@ -34,7 +35,7 @@ __device__ inline DVAE_GLOBAL T* as_global(const void* p) { return (DVAE_GLOBAL 
 
 constexpr float NS_SX = 16384.f, NS_SA = 8192.f, NS_SB = 8192.f;
 
-enum { NS_NORM, NS_SPLIT, NS_GRAM, NS_SYM, NS_APPLY, NS_PHASES };
+enum { NS_NORM, NS_SPLIT, NS_GRAM, NS_GRAM_TILES, NS_SQUARE, NS_APPLY, NS_PHASES };
 
 struct NsJob {
     const void* x;            // source, or gradient
@@ -46,6 +47,7 @@ struct NsJob {
     int vec;                  // Muon: no matrix, a plain momentum step
     int part;                 // first of its norm partials
     int nchunk;               // of its norm
+    int kc;                   // lines of 32 columns a workgroup of the Gram phase sums
     float scale;              // Muon: factor of the step
 };
 
@@ -53,14 +55,14 @@ struct NsArgs {
     const int* first;         // [NS_PHASES][jp]: first workgroup of each job, INT_MAX beyond the last
     const NsJob* jobs;
     double* norm;             // partial sums of squares
-    float* part;              // partial products of the Gram phase
+    float* part;              // partial tiles of the symmetric products
     char* ws;
     int njobs, jp;
     int total;                // workgroups of this launch
     int turn;                 // which transposed copy is read
-    int kc;                   // Gram: lines of 32 columns a workgroup sums
     float a, b, c;
     double eps;
+    NsJob one;                // the job, where there is only one: no table then
     float mu, nu, lr, decay;  // momentum, 1 - momentum, step, 1 - step * weight decay: each rounded once from 64 bits
     int nesterov;
 };
@@ -83,6 +85,10 @@ __global__ __launch_bounds__(256) void ns_table_kernel(NsBlob blob, unsigned* ds
 
 // The job of a workgroup, found by a wave at once: how many firsts are not beyond it.
 __device__ inline int ns_find(const NsArgs& g, int phase, int wg, int& local) {
+    if (g.njobs == 1) {
+        local = wg;
+        return 0;
+    }
     const int* first = g.first + phase * g.jp;
     const int lane = threadIdx.x & 63;
     int job = -1, start = 0;
@@ -100,11 +106,16 @@ __device__ inline int ns_find(const NsArgs& g, int phase, int wg, int& local) {
     return __builtin_amdgcn_readfirstlane(job);
 }
 
+__device__ inline NsJob ns_job_of(const NsArgs& g, int job) { return g.njobs == 1 ? g.one : g.jobs[job]; }
+
 // Consecutive workgroups run on different XCDs; neighbouring tiles share operands and go to the same one's L2.
 __device__ inline int ns_swizzle(int id, int total) {
     const int per = total >> 3, whole = per << 3;
     return id < whole ? (id & 7) * per + (id >> 3) : id;
 }
+
+// A row's part of the line that holds column `col`: its first chunk.  Chunks lie 16 * rows bytes apart, h's in 0..3, l's in 4..7.
+__device__ inline gbytes ns_line(gbytes base, long rows, int row, int col) { return base + ((col >> 5) * rows * 8 + row) * 16; }
 
 struct NsPlanes {
     int P, Q;
@@ -148,7 +159,7 @@ template <typename T, bool MUON>
 __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs g) {
     __shared__ double red[4];
     int chunk;
-    const NsJob j = g.jobs[ns_find(g, NS_NORM, blockIdx.x, chunk)];
+    const NsJob j = ns_job_of(g, ns_find(g, NS_NORM, blockIdx.x, chunk));
     const long n = (long)j.m * j.n;
     const auto x = as_global<const T>(j.x);
     const auto mom = as_global<float>(j.mom), par = as_global<float>(j.out);
@@ -196,7 +207,7 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsArgs g) {
     __shared__ unsigned tile[64][65];
     __shared__ double red[4];
     int t;
-    const NsJob j = g.jobs[ns_find(g, NS_SPLIT, blockIdx.x, t)];
+    const NsJob j = ns_job_of(g, ns_find(g, NS_SPLIT, blockIdx.x, t));
     double s = 0.0;
     for (int i = threadIdx.x; i < j.nchunk; i += 256) s += g.norm[j.part + i];
 #pragma unroll
@@ -222,12 +233,12 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsArgs g) {
         tile[i * 4 + wave][lane] = ns_split(v);
     }
     __syncthreads();
-    // a thread writes 16 columns of a row: first in the source's orientation, then in the other
+    // a wave writes 16 columns of 64 rows: first in the source's orientation, then in the other
 #pragma unroll
     for (int flip = 0; flip < 2; ++flip) {
         gbytes dst = flip ? (tall ? w.x : w.xt0) : (tall ? w.xt0 : w.x);
         const long rows = ns_pad(flip ? j.n : j.m);
-        const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 16;
+        const int r = lane, c = wave * 16;
         unsigned h[8], l[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -237,26 +248,41 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsArgs g) {
             l[i] = (u0 >> 16) | (u1 & 0xffff0000u);
         }
         const int row = (flip ? c0 : r0) + r, col = (flip ? r0 : c0) + c;
-        gbytes p = dst + ((col >> 5) * rows + row) * 128 + (col & 31) * 2;
-        *(DVAE_GLOBAL u32x4*)(p) = u32x4{h[0], h[1], h[2], h[3]};
-        *(DVAE_GLOBAL u32x4*)(p + 16) = u32x4{h[4], h[5], h[6], h[7]};
-        *(DVAE_GLOBAL u32x4*)(p + 64) = u32x4{l[0], l[1], l[2], l[3]};
-        *(DVAE_GLOBAL u32x4*)(p + 80) = u32x4{l[4], l[5], l[6], l[7]};
+        const gbytes p = ns_line(dst, rows, row, col) + (col & 31) / 8 * rows * 16;
+        *(DVAE_GLOBAL u32x4*)p = u32x4{h[0], h[1], h[2], h[3]};
+        *(DVAE_GLOBAL u32x4*)(p + rows * 16) = u32x4{h[4], h[5], h[6], h[7]};
+        *(DVAE_GLOBAL u32x4*)(p + rows * 64) = u32x4{l[0], l[1], l[2], l[3]};
+        *(DVAE_GLOBAL u32x4*)(p + rows * 80) = u32x4{l[4], l[5], l[6], l[7]};
     }
+}
+
+// what lanes of a wave wrote to LDS is there for its other lanes
+__device__ inline void ns_wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 // ---- the products ----------------------------------------------------------------------------------------------------
 // C[i][k] = sum over c of L[i][c] R[k][c] for a TS x TS tile: four waves, a quarter tile each, 32x32x16 MFMAs.  Two LDS
 // stages of one line (32 columns) per row, one barrier a line: while one half of a line is multiplied, the fragments of the
-// other half are on their way from LDS, and the lines after next are on their way from memory in two sets of registers.
+// other half are on their way from LDS, and the next lines are on their way from memory in sets of registers.
 // A line's eight 16-byte chunks are stored at chunk ^ (row / 2 & 7): of a fragment's rows any sixteen that are read at a time
 // meet the 64 banks once each.
-template <int TS>
+//
+// Two groups (G) of four waves share the contraction of one tile, each with stages of its own, and add up at the end (join): with
+// no more tiles than CUs a CU has two waves a SIMD to cover each other's waits all the same.
+template <int TS, int G = 1>
 struct NsTile {
     static constexpr int S = TS / 64;                    // subtiles of a wave each way
     static constexpr int PASS = TS / 32;                 // passes of 256 threads over a stage of one operand
-    static constexpr int BYTES = 2 * 2 * TS * 128;
+    static constexpr int STAGES = 2 * 2 * TS * 128;      // bytes of a group
+    static constexpr int BYTES = G * STAGES;
+    static constexpr int AHEAD = 2;                      // lines on their way from memory
     f32x16 acc[S][S];
+    // A dependent MFMA waits for two times its issue: a wave with a single subtile sums its three products apart.
+    f32x16 side[2];
+    int from = 0, to = S;                                // rows of subtiles that are this group's after join
 
     struct Lines { u32x4 l[PASS], r[PASS]; };
     struct Frags { f16x8 lh[S], ll[S], rh[S], rl[S]; };
@@ -268,6 +294,7 @@ struct NsTile {
             for (int k = 0; k < S; ++k)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[i][k][e] = 0.f;
+        side[0] = side[1] = acc[0][0];
     }
 
     // MFMAs FROM to TO of the 3 S^2 of half a line
@@ -276,20 +303,32 @@ struct NsTile {
 #pragma unroll
         for (int m = FROM; m < TO; ++m) {
             const int w = m / (S * S), i = m / S % S, n = m % S;
-            acc[i][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w == 1 ? f.ll[i] : f.lh[i], w == 0 ? f.rl[n] : f.rh[n], acc[i][n], 0, 0, 0);
+            f32x16& to = S == 1 && w < 2 ? side[w] : acc[i][n];
+            to = __builtin_amdgcn_mfma_f32_32x32x16_f16(w == 1 ? f.ll[i] : f.lh[i], w == 0 ? f.rl[n] : f.rh[n], to, 0, 0, 0);
         }
     }
     // `lines` is even; rows past lrows / rrows re-read the last one: their results are not stored
     __device__ inline void run(cgbytes L, int lrows, int l0, cgbytes R, int rrows, int r0, int line0, int lines, char* smem) {
-        const int tid = threadIdx.x, row = tid >> 3, chunk = tid & 7;
+        const int tid = threadIdx.x & 255, row = tid & 31, chunk = tid >> 5, group = threadIdx.x >> 8;
         const int lane = tid & 63, wave = tid >> 6;
+        if (G > 1) {
+            // where the lines do not make an even number for each, the first group takes all and the other keeps the barriers' count
+            const int active = lines % (2 * G) == 0 ? G : 1;
+            lines /= active;
+            if (group >= active) {
+                for (int k = 0; k <= lines; ++k) __syncthreads();
+                return;
+            }
+            line0 += group * lines;
+            smem += group * STAGES;
+        }
         cgbytes lp[PASS], rp[PASS];
 #pragma unroll
         for (int i = 0; i < PASS; ++i) {
-            lp[i] = L + ((long)line0 * lrows + min(l0 + i * 32 + row, lrows - 1)) * 128 + chunk * 16;
-            rp[i] = R + ((long)line0 * rrows + min(r0 + i * 32 + row, rrows - 1)) * 128 + chunk * 16;
+            lp[i] = L + (((long)line0 * 8 + chunk) * lrows + min(l0 + i * 32 + row, lrows - 1)) * 16;
+            rp[i] = R + (((long)line0 * 8 + chunk) * rrows + min(r0 + i * 32 + row, rrows - 1)) * 16;
         }
-        Lines set[2];
+        Lines set[AHEAD];
         int ahead = lines;
         auto fetch = [&](Lines& s) {                      // the next line; past the last one, that one again
 #pragma unroll
@@ -330,41 +369,75 @@ struct NsTile {
             }
         };
         Frags f0, f1;
-        fetch(set[0]);
-        fetch(set[1]);
+#pragma unroll
+        for (int d = 0; d < AHEAD; ++d) fetch(set[d]);
         stage(0, set[0]);
         fetch(set[0]);
         __syncthreads();
         read(f0, 0, 0);
-        for (int k = 0; k < lines; k += 2) {
+        for (int k = 0; k < lines; k += AHEAD) {
 #pragma unroll
-            for (int d = 0; d < 2; ++d) {
-                read(f1, d, 1);
+            for (int d = 0; d < AHEAD; ++d) {
+                const int next = (d + 1) % AHEAD;
+                read(f1, d & 1, 1);
                 multiply<0, S * S>(f0);
-                stage(d ^ 1, set[d ^ 1]);
+                stage((d & 1) ^ 1, set[next]);
                 multiply<S * S, 3 * S * S>(f0);
-                fetch(set[d ^ 1]);
+                fetch(set[next]);
                 multiply<0, S * S>(f1);
                 __syncthreads();                          // this line's fragments are out, the next line is in
-                read(f0, d ^ 1, 0);
+                read(f0, (d & 1) ^ 1, 0);
                 multiply<S * S, 3 * S * S>(f1);
             }
         }
+        if (S == 1) acc[0][0] += side[0] + side[1];
+    }
+
+    // Adds the groups up: each keeps a row of subtiles.
+    __device__ inline void join(char* smem) {
+        static_assert(G == 1 || (G == 2 && S == 2), "two groups, two rows of subtiles");
+        if (G == 1) return;
+        const int tid = threadIdx.x & 255, group = threadIdx.x >> 8;
+        __syncthreads();                                  // the stages are read
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            if (i == group) continue;
+#pragma unroll
+            for (int k = 0; k < S; ++k)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<f32x4*>(smem + group * STAGES + ((k * 4 + q) * 256 + tid) * 16) =
+                        f32x4{acc[i][k][4 * q], acc[i][k][4 * q + 1], acc[i][k][4 * q + 2], acc[i][k][4 * q + 3]};
+        }
+        __syncthreads();
+        from = group;
+        to = group + 1;
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            if (i != group) continue;
+#pragma unroll
+            for (int k = 0; k < S; ++k)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const f32x4 v = *reinterpret_cast<const f32x4*>(smem + (group ^ 1) * STAGES + ((k * 4 + q) * 256 + tid) * 16);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][k][4 * q + e] += v[e];
+                }
+        }
+        __syncthreads();                                  // before the patches of the stores
     }
 
     // of element e of subtile (i, k): row and column inside the tile
     __device__ static inline int row_of(int i, int e) {
-        return (threadIdx.x >> 7) * (TS / 2) + i * 32 + 8 * (e >> 2) + 4 * ((threadIdx.x >> 5) & 1) + (e & 3);
+        return (threadIdx.x >> 7 & 1) * (TS / 2) + i * 32 + 8 * (e >> 2) + 4 * ((threadIdx.x >> 5) & 1) + (e & 3);
     }
     __device__ static inline int col_of(int k) { return ((threadIdx.x >> 6) & 1) * (TS / 2) + k * 32 + (threadIdx.x & 31); }
 };
 
-// the line of a row that holds column `col`, a multiple of 32
-__device__ inline gbytes ns_line(gbytes base, int rows, int row, int col) { return base + ((long)(col >> 5) * rows + row) * 128; }
-
-// A 32x32 subtile (already scaled) to plane pairs: along its rows at `dst` (through a per-wave LDS patch) and, transposed,
-// at `dst_t` straight from the registers, where a lane holds four consecutive rows of one column.  Either may be NULL.
-__device__ inline void ns_store(const f32x16& v, unsigned* patch, gbytes dst, gbytes dst_t) {
+// A 32x32 subtile (already scaled) to plane pairs: along its rows at `dst`, of an operand of `rows` rows (through a per-wave LDS
+// patch), and, transposed, at `dst_t` straight from the registers, where a lane holds four consecutive rows of one column,
+// half a chunk.  Either may be NULL.
+__device__ inline void ns_store(const f32x16& v, unsigned* patch, gbytes dst, long rows, gbytes dst_t, long rows_t) {
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
     unsigned u[16];
 #pragma unroll
@@ -372,31 +445,28 @@ __device__ inline void ns_store(const f32x16& v, unsigned* patch, gbytes dst, gb
     if (dst_t) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            gbytes p = dst_t + col * 128 + (8 * q + 4 * half) * 2;
+            const gbytes p = dst_t + (q * rows_t + col) * 16 + half * 8;
             const unsigned* w = u + 4 * q;
-            *(DVAE_GLOBAL u32x2*)(p) = u32x2{(w[0] & 0xffffu) | (w[1] << 16), (w[2] & 0xffffu) | (w[3] << 16)};
-            *(DVAE_GLOBAL u32x2*)(p + 64) = u32x2{(w[0] >> 16) | (w[1] & 0xffff0000u), (w[2] >> 16) | (w[3] & 0xffff0000u)};
+            *(DVAE_GLOBAL u32x2*)p = u32x2{(w[0] & 0xffffu) | (w[1] << 16), (w[2] & 0xffffu) | (w[3] << 16)};
+            *(DVAE_GLOBAL u32x2*)(p + rows_t * 64) = u32x2{(w[0] >> 16) | (w[1] & 0xffff0000u), (w[2] >> 16) | (w[3] & 0xffff0000u)};
         }
     }
     if (dst) {
         constexpr int ST = 36;
 #pragma unroll
         for (int e = 0; e < 16; ++e) patch[(8 * (e >> 2) + 4 * half + (e & 3)) * ST + col] = u[e];
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        ns_wave_sync();
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            const int r = (lane >> 2) + 16 * k, c = (lane & 3) * 8;
-            const u32x4 a = *reinterpret_cast<const u32x4*>(patch + r * ST + c), b = *reinterpret_cast<const u32x4*>(patch + r * ST + c + 4);
-            gbytes p = dst + r * 128 + c * 2;
-            *(DVAE_GLOBAL u32x4*)(p) = u32x4{(a[0] & 0xffffu) | (a[1] << 16), (a[2] & 0xffffu) | (a[3] << 16),
-                                                 (b[0] & 0xffffu) | (b[1] << 16), (b[2] & 0xffffu) | (b[3] << 16)};
-            *(DVAE_GLOBAL u32x4*)(p + 64) = u32x4{(a[0] >> 16) | (a[1] & 0xffff0000u), (a[2] >> 16) | (a[3] & 0xffff0000u),
-                                                      (b[0] >> 16) | (b[1] & 0xffff0000u), (b[2] >> 16) | (b[3] & 0xffff0000u)};
+            const int r = (lane & 15) + 16 * k, c = lane >> 4;
+            const u32x4 a = *reinterpret_cast<const u32x4*>(patch + r * ST + c * 8), b = *reinterpret_cast<const u32x4*>(patch + r * ST + c * 8 + 4);
+            const gbytes p = dst + (c * rows + r) * 16;
+            *(DVAE_GLOBAL u32x4*)p = u32x4{(a[0] & 0xffffu) | (a[1] << 16), (a[2] & 0xffffu) | (a[3] << 16),
+                                           (b[0] & 0xffffu) | (b[1] << 16), (b[2] & 0xffffu) | (b[3] << 16)};
+            *(DVAE_GLOBAL u32x4*)(p + rows * 64) = u32x4{(a[0] >> 16) | (a[1] & 0xffff0000u), (a[2] >> 16) | (a[3] & 0xffff0000u),
+                                                         (b[0] >> 16) | (b[1] & 0xffff0000u), (b[2] >> 16) | (b[3] & 0xffff0000u)};
         }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        ns_wave_sync();
     }
 }
 
@@ -410,171 +480,256 @@ __device__ inline void ns_triangle(int t, int& i, int& k) {
 
 // The symmetric products store the tiles at and below the diagonal and their mirror images.  Tiles on the diagonal are
 // stored once: their two halves agree to rounding only, and two writers of one place would leave either's.
-template <int TS>
-__device__ inline void ns_store_symmetric(NsTile<TS>& c, char* smem, gbytes dst, int P, int ti, int tk) {
+template <int TS, int G>
+__device__ inline void ns_store_symmetric(NsTile<TS, G>& c, char* smem, gbytes dst, int P, int ti, int tk) {
     constexpr int S = NsTile<TS>::S;
-    const int wave = threadIdx.x >> 6, wr = (wave >> 1) * (TS / 2), wc = (wave & 1) * (TS / 2);
+    const int wave = threadIdx.x >> 6, wr = (wave >> 1 & 1) * (TS / 2), wc = (wave & 1) * (TS / 2);
     unsigned* patch = reinterpret_cast<unsigned*>(smem) + wave * (32 * 36);
 #pragma unroll
     for (int i = 0; i < S; ++i)
 #pragma unroll
         for (int k = 0; k < S; ++k) {
             const int row = ti * TS + wr + i * 32, col = tk * TS + wc + k * 32;
-            if (row >= P || col >= P) continue;
-            ns_store(c.acc[i][k], patch, ns_line(dst, P, row, col), ti != tk ? ns_line(dst, P, col, row) : gbytes(nullptr));
+            if (row >= P || col >= P || i < c.from || i >= c.to) continue;
+            ns_store(c.acc[i][k], patch, ns_line(dst, P, row, col), P, ti != tk ? ns_line(dst, P, col, row) : gbytes(nullptr), P);
         }
 }
 
-// A = X X^T, whole or, where the tiles alone would leave most of the chip idle, in `kc`-line pieces of the contraction that
-// leave fp32 partial tiles for ns_gram_sum_kernel.
-template <int TS, bool PIECES>
-__global__ __launch_bounds__(256, 2) void ns_gram_kernel(NsArgs g) {
-    __shared__ __align__(16) char smem[NsTile<TS>::BYTES];
+// Element e of four of B, from A^2 (scaled), from A's pieces and from whether it lies on the diagonal.
+__device__ inline float ns_polynomial(const NsArgs& g, float square, u32x2 h, u32x2 l, int e, bool diagonal) {
+    const f16x2 hv = __builtin_bit_cast(f16x2, (unsigned)h[e >> 1]), lv = __builtin_bit_cast(f16x2, (unsigned)l[e >> 1]);
+    float r = g.c * (NS_SB / (NS_SA * NS_SA)) * square + g.b * (NS_SB / NS_SA) * ((float)hv[e & 1] + (float)lv[e & 1]);
+    if (diagonal) r += g.a * NS_SB;
+    return r;
+}
+
+// What a symmetric product's subtile becomes: A = X X^T, or B = a I + b A + c A^2.  A lane's elements lie in column `col`, from
+// `row` on; those of A that B needs are read along row `col`, A being symmetric.
+template <bool SQUARE>
+__device__ inline void ns_symmetric_value(const NsArgs& g, const NsPlanes& w, f32x16& v, int row, int col) {
+    if (!SQUARE) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] *= NS_SA / (NS_SX * NS_SX);
+        return;
+    }
+    const long rows = w.P;
+    const cgbytes p = ns_line(w.a, rows, col, row & ~31) + (row & 4) * 2;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const u32x2 h = *(const DVAE_GLOBAL u32x2*)(p + q * rows * 16), l = *(const DVAE_GLOBAL u32x2*)(p + (4 + q) * rows * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * q + e] = ns_polynomial(g, v[4 * q + e], h, l, e, row + 8 * q + e == col);
+    }
+}
+
+// The symmetric products, tiles at and below the diagonal: whole or (Gram, where the tiles alone would leave much of the chip
+// idle) in pieces of the contraction, a job's kc lines each, that leave fp32 partial tiles for ns_gram_sum_kernel.  Neighbouring
+// workgroups take different tiles of the same lines: an XCD reads a part of X once.
+template <int TS, bool SQUARE, bool PIECES, int G>
+__global__ __launch_bounds__(256 * G, G == 1 ? 2 : 1) void ns_symmetric_kernel(NsArgs g) {
+    extern __shared__ __align__(16) char smem[];
     constexpr int S = NsTile<TS>::S;
-    int t;
+    int t, ti, tk;
     const int wg = ns_swizzle(blockIdx.x, g.total);
-    const NsJob j = g.jobs[ns_find(g, NS_GRAM, wg, t)];
+    const NsJob j = ns_job_of(g, ns_find(g, SQUARE ? NS_SQUARE : NS_GRAM, wg, t));
     const NsPlanes w(g, j);
-    const int lines = w.Q / 32, pieces = PIECES ? (lines + g.kc - 1) / g.kc : 1;
-    int ti, tk;
-    ns_triangle(t / pieces, ti, tk);
-    const int line0 = PIECES ? t % pieces * g.kc : 0;
-    NsTile<TS> c;
+    const int side = (w.P + TS - 1) / TS, tiles = side * (side + 1) / 2;
+    const int lines = (SQUARE ? w.P : w.Q) / 32, kc = j.kc, line0 = PIECES ? t / tiles * kc : 0;
+    ns_triangle(PIECES ? t % tiles : t, ti, tk);
+    NsTile<TS, G> c;
     c.zero();
-    c.run(w.x, w.P, ti * TS, w.x, w.P, tk * TS, line0, PIECES ? min(g.kc, lines - line0) : lines, smem);
+    const cgbytes m = SQUARE ? w.a : w.x;
+    c.run(m, w.P, ti * TS, m, w.P, tk * TS, line0, PIECES ? min(kc, lines - line0) : lines, smem);
+    c.join(smem);
     if (PIECES) {
-        float* out = g.part + (long)wg * (TS * TS) + threadIdx.x;
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+        const auto out = as_global<float>(g.part) + (long)wg * (TS * TS) + lane * 4;
 #pragma unroll
         for (int i = 0; i < S; ++i)
 #pragma unroll
             for (int k = 0; k < S; ++k)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) out[((i * S + k) * 16 + e) * 256] = c.acc[i][k][e];
+                for (int q = 0; q < 4; ++q) {
+                    // subtile (row block, column block) of the tile, then its quarters, a lane's four values together
+                    const int sub = ((wave >> 1) * S + i) * (2 * S) + (wave & 1) * S + k;
+                    *(DVAE_GLOBAL f32x4*)(out + (sub * 4 + q) * 256) = f32x4{c.acc[i][k][4 * q], c.acc[i][k][4 * q + 1], c.acc[i][k][4 * q + 2], c.acc[i][k][4 * q + 3]};
+                }
         return;
     }
 #pragma unroll
     for (int i = 0; i < S; ++i)
 #pragma unroll
-        for (int k = 0; k < S; ++k)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) c.acc[i][k][e] *= NS_SA / (NS_SX * NS_SX);
-    ns_store_symmetric<TS>(c, smem, w.a, w.P, ti, tk);
+        for (int k = 0; k < S; ++k) {
+            const int row = ti * TS + NsTile<TS>::row_of(i, 0), col = tk * TS + NsTile<TS>::col_of(k);
+            if (row < w.P && col < w.P && i >= c.from && i < c.to) ns_symmetric_value<SQUARE>(g, w, c.acc[i][k], row, col);
+        }
+    ns_store_symmetric(c, smem, SQUARE ? w.b : w.a, w.P, ti, tk);
 }
 
+// Adds the pieces up, a workgroup for each 32x32 subtile: its waves take every fourth piece, four in flight, always in the same order.
 template <int TS>
 __global__ __launch_bounds__(256) void ns_gram_sum_kernel(NsArgs g) {
-    __shared__ __align__(16) char smem[4 * 32 * 36 * 4];
-    constexpr int S = NsTile<TS>::S;
-    int t;
-    const int jn = ns_find(g, NS_SYM, blockIdx.x, t);
-    const NsJob j = g.jobs[jn];
+    constexpr int SUBS = (TS / 32) * (TS / 32);
+    __shared__ f32x4 red[3][4][64];
+    __shared__ unsigned patch[32 * 36];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int sub = blockIdx.x % SUBS;
+    int t, ti, tk;
+    const int jn = ns_find(g, NS_GRAM_TILES, blockIdx.x / SUBS, t);
+    const NsJob j = ns_job_of(g, jn);
     const NsPlanes w(g, j);
-    const int pieces = (w.Q / 32 + g.kc - 1) / g.kc;
-    const float* in = g.part + ((long)g.first[NS_GRAM * g.jp + jn] + (long)t * pieces) * (TS * TS) + threadIdx.x;
-    NsTile<TS> c;
-    c.zero();
-    static_assert(S == 1, "pieces are cut for tiles of 64");
-    for (int s = 0; s < pieces; s += 4, in += 4 * TS * TS) {          // four pieces' loads in flight
-        float v[4][16];
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) v[u][e] = s + u < pieces ? in[u * TS * TS + e * 256] : 0.f;
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) c.acc[0][0][e] += v[u][e];
-    }
-#pragma unroll
-    for (int i = 0; i < S; ++i)
-#pragma unroll
-        for (int k = 0; k < S; ++k)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) c.acc[i][k][e] *= NS_SA / (NS_SX * NS_SX);
-    int ti, tk;
     ns_triangle(t, ti, tk);
-    ns_store_symmetric<TS>(c, smem, w.a, w.P, ti, tk);
+    const int row = ti * TS + sub / (TS / 32) * 32, col = tk * TS + sub % (TS / 32) * 32;
+    if (row >= w.P || col >= w.P) return;
+    const int side = (w.P + TS - 1) / TS, tiles = side * (side + 1) / 2;
+    const int pieces = (w.Q / 32 + j.kc - 1) / j.kc;
+    const auto in = as_global<const float>(g.part) + ((g.njobs == 1 ? 0L : (long)g.first[NS_GRAM * g.jp + jn]) + t) * (TS * TS) + sub * 1024 + lane * 4;
+    f32x4 v[4] = {};
+    for (int s = wave; s < pieces; s += 16) {
+        f32x4 r[4][4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) r[u][q] = *(const DVAE_GLOBAL f32x4*)(in + (long)min(s + 4 * u, pieces - 1) * tiles * (TS * TS) + q * 256);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (s + 4 * u < pieces) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) v[q] += r[u][q];
+            }
+    }
+    if (wave) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) red[wave - 1][q][lane] = v[q];
+    }
+    __syncthreads();
+    if (wave) return;
+    f32x16 a;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const f32x4 f = (v[q] + red[0][q][lane]) + (red[1][q][lane] + red[2][q][lane]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[4 * q + e] = f[e];
+    }
+    ns_symmetric_value<false>(g, w, a, row + 4 * (lane >> 5), col + (lane & 31));
+    ns_store(a, patch, ns_line(w.a, w.P, row, col), w.P, ti != tk ? ns_line(w.a, w.P, col, row) : gbytes(nullptr), w.P);
 }
 
-// B = a I + b A + c A^2
-template <int TS>
-__global__ __launch_bounds__(256, 2) void ns_square_kernel(NsArgs g) {
-    __shared__ __align__(16) char smem[NsTile<TS>::BYTES];
-    constexpr int S = NsTile<TS>::S;
+// B = a I + b A + c A^2 for matrices whose A is small against the chip: tiles of 32, a workgroup each, so that many CUs fetch; its
+// four waves take every fourth line and feed their MFMAs straight from memory (a tile's rows are read once a workgroup: LDS would
+// only add its latency and a barrier a line).  What is left is a chain of four latencies: 36 tiles of 64 take 8.2 us for p = 512,
+// 136 of these %D512%.
+__global__ __launch_bounds__(256, 2) void ns_square_small_kernel(NsArgs g) {
+    __shared__ f32x4 red[4][4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     int t, ti, tk;
-    const NsJob j = g.jobs[ns_find(g, NS_SYM, ns_swizzle(blockIdx.x, g.total), t)];
+    const NsJob j = ns_job_of(g, ns_find(g, NS_SQUARE, blockIdx.x, t));
     const NsPlanes w(g, j);
     ns_triangle(t, ti, tk);
-    NsTile<TS> c;
-    c.zero();
-    c.run(w.a, w.P, ti * TS, w.a, w.P, tk * TS, 0, w.P / 32, smem);
-    const float s2 = g.c * (NS_SB / (NS_SA * NS_SA)), s1 = g.b * (NS_SB / NS_SA), s0 = g.a * NS_SB;
+    const int lines = w.P / 32;
+    const long rows = w.P;
+    const cgbytes lp = ns_line(w.a, rows, ti * 32 + (lane & 31), 0) + half * rows * 16, rp = ns_line(w.a, rows, tk * 32 + (lane & 31), 0) + half * rows * 16;
+    f32x16 acc[3];
 #pragma unroll
-    for (int i = 0; i < S; ++i)
+    for (int k = 0; k < 3; ++k)
 #pragma unroll
-        for (int k = 0; k < S; ++k) {
-            const int col = tk * TS + NsTile<TS>::col_of(k), row = ti * TS + NsTile<TS>::row_of(i, 0);
-            if (col >= w.P || row >= w.P) continue;
-            // a lane's elements of A lie along a column: read as a row, A being symmetric
-            cgbytes p = ns_line(w.a, w.P, col, row & ~31) + (row & 31) * 2;
+        for (int e = 0; e < 16; ++e) acc[k][e] = 0.f;
+    // this wave's quarter of the tile at the end: rows row .. row + 3 of column col, that is of A's row col
+    const int row = ti * 32 + 8 * wave + 4 * half, col = tk * 32 + (lane & 31);
+    const cgbytes own = ns_line(w.a, rows, col, ti * 32) + wave * rows * 16 + half * 8;
+    u32x2 oh, ol;
+    for (int line = wave; line < lines; line += 16) {
+        f16x8 l[4][4], r[4][4];                           // [line][two halves of h, then of l]; past the last line that one again, unused
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const u32x2 h = *(const DVAE_GLOBAL u32x2*)(p + 16 * q), l = *(const DVAE_GLOBAL u32x2*)(p + 16 * q + 64);
+        for (int u = 0; u < 4; ++u)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const f16x2 hv = __builtin_bit_cast(f16x2, (unsigned)h[e >> 1]), lv = __builtin_bit_cast(f16x2, (unsigned)l[e >> 1]);
-                    const float av = (float)hv[e & 1] + (float)lv[e & 1];
-                    float r = s2 * c.acc[i][k][4 * q + e] + s1 * av;
-                    if (row + 8 * q + e == col) r += s0;
-                    c.acc[i][k][4 * q + e] = r;
-                }
+            for (int c = 0; c < 4; ++c) {
+                const long at = (min(line + 4 * u, lines - 1) * 8 + c * 2) * rows * 16;
+                l[u][c] = *(const DVAE_GLOBAL f16x8*)(lp + at);
+                r[u][c] = *(const DVAE_GLOBAL f16x8*)(rp + at);
+            }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (line + 4 * u >= lines) break;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[u][k], r[u][2 + k], acc[0], 0, 0, 0);
+                acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[u][2 + k], r[u][k], acc[1], 0, 0, 0);
+                acc[2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[u][k], r[u][k], acc[2], 0, 0, 0);
             }
         }
-    ns_store_symmetric<TS>(c, smem, w.b, w.P, ti, tk);
+    }
+    oh = *(const DVAE_GLOBAL u32x2*)own;
+    ol = *(const DVAE_GLOBAL u32x2*)(own + rows * 64);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[0][4 * q + e] + acc[1][4 * q + e] + acc[2][4 * q + e];
+        red[wave][q][lane] = v;
+    }
+    __syncthreads();
+    const f32x4 v = (red[0][wave][lane] + red[1][wave][lane]) + (red[2][wave][lane] + red[3][wave][lane]);
+    unsigned u[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[e] = ns_split(ns_polynomial(g, v[e], oh, ol, e, row + e == col));
+    const gbytes dst = ns_line(w.b, rows, col, ti * 32) + wave * rows * 16 + half * 8;
+    *(DVAE_GLOBAL u32x2*)dst = u32x2{(u[0] & 0xffffu) | (u[1] << 16), (u[2] & 0xffffu) | (u[3] << 16)};
+    *(DVAE_GLOBAL u32x2*)(dst + rows * 64) = u32x2{(u[0] >> 16) | (u[1] & 0xffff0000u), (u[2] >> 16) | (u[3] & 0xffff0000u)};
+    if (ti != tk) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const gbytes p = ns_line(w.b, rows, row + e, tk * 32) + (lane >> 3 & 3) * rows * 16 + (lane & 7) * 2;
+            *(DVAE_GLOBAL unsigned short*)p = (unsigned short)u[e];
+            *(DVAE_GLOBAL unsigned short*)(p + rows * 64) = (unsigned short)(u[e] >> 16);
+        }
+    }
 }
 
 // X <- B X, left in both orientations
-template <int TS>
-__global__ __launch_bounds__(256, 2) void ns_apply_kernel(NsArgs g) {
-    __shared__ __align__(16) char smem[NsTile<TS>::BYTES];
+template <int TS, int G>
+__global__ __launch_bounds__(256 * G, G == 1 ? 2 : 1) void ns_apply_kernel(NsArgs g) {
+    extern __shared__ __align__(16) char smem[];
     constexpr int S = NsTile<TS>::S;
     int t;
-    const NsJob j = g.jobs[ns_find(g, NS_APPLY, ns_swizzle(blockIdx.x, g.total), t)];
+    const NsJob j = ns_job_of(g, ns_find(g, NS_APPLY, ns_swizzle(blockIdx.x, g.total), t));
     const NsPlanes w(g, j);
     const int ni = (w.P + TS - 1) / TS, ti = t % ni, tk = t / ni;
-    NsTile<TS> c;
+    NsTile<TS, G> c;
     c.zero();
     c.run(w.b, w.P, ti * TS, w.xt(g.turn), w.Q, tk * TS, 0, w.P / 32, smem);
-    const int wave = threadIdx.x >> 6, wr = (wave >> 1) * (TS / 2), wc = (wave & 1) * (TS / 2);
+    c.join(smem);
+    const int wave = threadIdx.x >> 6, wr = (wave >> 1 & 1) * (TS / 2), wc = (wave & 1) * (TS / 2);
     unsigned* patch = reinterpret_cast<unsigned*>(smem) + wave * (32 * 36);
 #pragma unroll
     for (int i = 0; i < S; ++i)
 #pragma unroll
         for (int k = 0; k < S; ++k) {
             const int row = ti * TS + wr + i * 32, col = tk * TS + wc + k * 32;
-            if (row >= w.P || col >= w.Q) continue;
+            if (row >= w.P || col >= w.Q || i < c.from || i >= c.to) continue;
 #pragma unroll
             for (int e = 0; e < 16; ++e) c.acc[i][k][e] *= 1.f / NS_SB;
-            ns_store(c.acc[i][k], patch, ns_line(w.x, w.P, row, col), ns_line(w.xt(g.turn ^ 1), w.Q, col, row));
+            ns_store(c.acc[i][k], patch, ns_line(w.x, w.P, row, col), w.P, ns_line(w.xt(g.turn ^ 1), w.Q, col, row), w.Q);
         }
 }
 
 // The last product: its tile goes to the caller's matrix, or steps the parameter.  A tall matrix's tile is computed
 // transposed (the operands trade places), so that lanes run along the caller's rows either way.
-template <int TS, typename T, bool MUON>
-__global__ __launch_bounds__(256, 2) void ns_last_kernel(NsArgs g) {
-    __shared__ __align__(16) char smem[NsTile<TS>::BYTES];
+template <int TS, typename T, bool MUON, int G>
+__global__ __launch_bounds__(256 * G, G == 1 ? 2 : 1) void ns_last_kernel(NsArgs g) {
+    extern __shared__ __align__(16) char smem[];
     constexpr int S = NsTile<TS>::S;
     int t;
-    const NsJob j = g.jobs[ns_find(g, NS_APPLY, ns_swizzle(blockIdx.x, g.total), t)];
+    const NsJob j = ns_job_of(g, ns_find(g, NS_APPLY, ns_swizzle(blockIdx.x, g.total), t));
     const NsPlanes w(g, j);
     const bool tall = j.m > j.n;
     const int ni = (w.P + TS - 1) / TS, tp = t % ni, tq = t / ni;
-    NsTile<TS> c;
+    NsTile<TS, G> c;
     c.zero();
     const cgbytes L = tall ? w.xt(g.turn) : w.b, R = tall ? w.b : w.xt(g.turn);
     const int lrows = tall ? w.Q : w.P, rrows = tall ? w.P : w.Q, ti = tall ? tq : tp, tk = tall ? tp : tq;
     c.run(L, lrows, ti * TS, R, rrows, tk * TS, 0, w.P / 32, smem);
+    c.join(smem);
     const auto out = as_global<T>(j.out);
     const float step = MUON ? g.lr * j.scale : 0.f;
 #pragma unroll
@@ -582,7 +737,7 @@ __global__ __launch_bounds__(256, 2) void ns_last_kernel(NsArgs g) {
 #pragma unroll
         for (int k = 0; k < S; ++k) {
             const int col = tk * TS + NsTile<TS>::col_of(k);
-            if (col >= j.n) continue;
+            if (col >= j.n || i < c.from || i >= c.to) continue;
             float p[16];
             if (MUON) {
 #pragma unroll

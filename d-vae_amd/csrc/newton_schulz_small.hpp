@@ -40,13 +40,6 @@ struct NsSmallLds {
 // 16-byte chunk `chunk` of row `row` of line `line`
 __device__ inline int ns_small_at(int line, int row, int chunk) { return (line * 64 + row) * 128 + ((chunk ^ (row >> 1 & 7)) << 4); }
 
-// what lanes of a wave wrote to LDS is there for its other lanes
-__device__ inline void ns_wave_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 struct NsBlock {
     f16x8 h[2][2], l[2][2];                               // [32 rows of p][half of the block's q]
 };

@@ -43,7 +43,7 @@ def _forward(x, weight, bias, eps, save):
     c = x.shape[-1]
     x2 = _rows(x, c)
     rows = x2.shape[0]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if save else None
     if rows:
         weight, bias = _param(weight), _param(bias)
@@ -51,6 +51,31 @@ def _forward(x, weight, bias, eps, save):
         L.check(L.lib().dvae_layer_norm_fwd(x2.data_ptr(), x2.stride(0), L.ptr(weight), L.ptr(bias), y.data_ptr(), c, mean,
                                             mean + 4 * rows if save else None, rows, c, eps, _DTYPES[x.dtype], L.stream()))
     return y, stats
+
+
+def _backward(ctx, dy):
+    x, weight, stats = ctx.saved_tensors
+    want_x, want_w, want_b, _ = ctx.needs_input_grad
+    with L.on_device(x.device):
+        c = x.shape[-1]
+        x2, dy2 = _rows(x, c), _rows(dy, c)
+        rows, dtype, lib = x2.shape[0], _DTYPES[x.dtype], L.lib()
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format) if want_x else None
+        dw = torch.empty(c, device=x.device, dtype=torch.float32) if want_w else None
+        db = torch.empty(c, device=x.device, dtype=torch.float32) if want_b else None
+        ws, n = None, 0
+        if want_w or want_b:
+            n = lib.dvae_layer_norm_workspace_bytes(rows, c, dtype)
+            ws = torch.empty(n, device=x.device, dtype=torch.uint8)
+        weight = _param(weight)
+        mean = stats.data_ptr()
+        L.check(lib.dvae_layer_norm_bwd(dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0), L.ptr(weight), mean,
+                                        mean + 4 * rows, L.ptr(dx), c, L.ptr(dw), L.ptr(db), L.ptr(ws), n, rows, c, dtype,
+                                        L.stream()))
+    return dx, dw, db, None
+
+
+_backward_once = torch.autograd.function.once_differentiable(_backward)
 
 
 class _LayerNormFunction(torch.autograd.Function):
@@ -61,27 +86,9 @@ class _LayerNormFunction(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, stats = ctx.saved_tensors
-        want_x, want_w, want_b = ctx.needs_input_grad[:3]
-        with L.on_device(x.device):
-            c = x.shape[-1]
-            x2, dy2 = _rows(x, c), _rows(dy, c)
-            rows, dtype = x2.shape[0], _DTYPES[x.dtype]
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_x else None
-            dw = torch.empty(c, dtype=torch.float32, device=x.device) if want_w else None
-            db = torch.empty(c, dtype=torch.float32, device=x.device) if want_b else None
-            ws, n = None, 0
-            if want_w or want_b:
-                n = L.lib().dvae_layer_norm_workspace_bytes(rows, c, dtype)
-                ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-            weight = _param(weight)
-            mean = stats.data_ptr()
-            L.check(L.lib().dvae_layer_norm_bwd(dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0), L.ptr(weight), mean,
-                                                mean + 4 * rows, L.ptr(dx), c, L.ptr(dw), L.ptr(db), L.ptr(ws), n, rows, c, dtype,
-                                                L.stream()))
-        return dx, dw, db, None
+        # the guard against second derivatives costs a third of a small call's backward: only where a graph is being built
+        return _backward_once(ctx, dy) if torch.is_grad_enabled() else _backward(ctx, dy)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
