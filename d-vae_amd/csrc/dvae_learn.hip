@@ -274,7 +274,9 @@ int ns_plan(const char* what, const dvae_matrix* mats, int count, int scale_rule
         longest[1] = longest[1] > P / 32 ? longest[1] : P / 32;
         p.matrices = true;
     }
-    p.gram_ts = cost[0][1] < cost[0][0] ? 128 : 64;
+    // The Gram product is cut into pieces anyhow: 128 once that leaves each of 512 workgroups eight lines (below, their starts and
+    // partial tiles cost more: 512 x 4608 210 us against 231, ResNet-18's matrices 575 against 560).
+    p.gram_ts = cost[0][1] < cost[0][0] && lines[1] >= 4096 ? 128 : 64;
     // a product of one tile a workgroup: 128 only where that still gives every CU one
     p.apply_ts = cost[2][1] < cost[2][0] && cost[2][1] / 256 >= 0.9 * (longest[1] * 0.78 + 3.0) ? 128 : 64;
     // The Gram product in pieces: about 512 workgroups, two a CU, of at least 4 lines; none where tiles of 64 alone are as many
