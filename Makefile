@@ -6,9 +6,10 @@ CSRC := $(PKG)/csrc
 LIB := $(PKG)/lib/libdvae_hip.so
 LEARN_HDRS := $(CSRC)/layer_norm.hpp $(CSRC)/newton_schulz.hpp $(CSRC)/newton_schulz_small.hpp
 HDRS := $(filter-out $(LEARN_HDRS),$(wildcard $(CSRC)/*.hpp)) include/dvae_hip.h
-FLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -fno-gpu-rdc -Wall -Wno-unused-function -mllvm -pragma-unroll-threshold=1000000
-# no packed fp32 arithmetic in the kernels (the host pass does not know the feature and says so)
-NO_PK := -Xclang -target-feature -Xclang -packed-fp32-ops
+# No packed fp32 arithmetic in the kernels: some of its forms have given wrong results now and then (the host pass does not know
+# the feature and says so).
+FLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -fno-gpu-rdc -Wall -Wno-unused-function -mllvm -pragma-unroll-threshold=1000000 \
+    -Xclang -target-feature -Xclang -packed-fp32-ops
 
 all: $(LIB)
 
@@ -18,7 +19,7 @@ $(PKG)/lib/dvae_hip.o: $(CSRC)/dvae_hip.hip $(HDRS)
 
 $(PKG)/lib/dvae_learn.o: $(CSRC)/dvae_learn.hip $(CSRC)/common.hpp $(LEARN_HDRS) include/dvae_hip.h
 	@mkdir -p $(PKG)/lib
-	$(HIPCC) $(FLAGS) $(NO_PK) -c -o $@ $<
+	$(HIPCC) $(FLAGS) -c -o $@ $<
 
 $(LIB): $(PKG)/lib/dvae_hip.o $(PKG)/lib/dvae_learn.o
 	$(HIPCC) --offload-arch=$(ARCH) -fPIC -shared -fno-gpu-rdc -o $@ $^
