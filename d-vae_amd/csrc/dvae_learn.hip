@@ -216,31 +216,51 @@ bool ns_all_small(const dvae_matrix* mats, int count) {
     return true;
 }
 
+// words of host memory to the device, as many kernel arguments at a time as fit
+int ns_upload(const char* what, const unsigned* words, size_t count, unsigned* dst, hipStream_t st) {
+    NsBlob blob;
+    for (size_t at = 0; at < count; at += NsBlob::WORDS) {
+        const size_t n = count - at < (size_t)NsBlob::WORDS ? count - at : (size_t)NsBlob::WORDS;
+        memcpy(blob.w, words + at, n * 4);
+        hipLaunchKernelGGL(ns_table_kernel, dim3(1), dim3(256), 0, st, blob, dst + at, (int)n);
+        DVAE_CHECK_LAUNCH(what);
+    }
+    return DVAE_OK;
+}
+
+size_t ns_small_bytes(int count) { return count <= NS_SMALL_JOBS ? 256 : align256(count * sizeof(NsJob)); }
+
+// A workgroup for each matrix: up to 32 in the kernel's arguments, more in a table.
 template <typename T, bool MUON>
 int ns_run_small(const char* what, const dvae_matrix* mats, int count, int scale_rule, const NsArgs& g, int steps, hipStream_t st) {
     static LdsOptIn opt[3];
     NsSmallArgs a{};
     a.eps = g.eps; a.a = g.a; a.b = g.b; a.c = g.c; a.mu = g.mu; a.nu = g.nu; a.lr = g.lr; a.decay = g.decay;
     a.nesterov = g.nesterov; a.steps = steps;
-    for (int i = 0; i < count; i += NS_SMALL_JOBS) {
-        const int some = count - i < NS_SMALL_JOBS ? count - i : NS_SMALL_JOBS;
-        int q = 1;
-        for (int k = 0; k < some; ++k) {
-            ns_job(mats[i + k], scale_rule, a.jobs[k]);
-            if (!a.jobs[k].vec) q = fmax(q, fmax(a.jobs[k].m, a.jobs[k].n));
-        }
-        const int lds = (int)sizeof(NsSmallLds);
+    std::vector<NsJob> many((size_t)(count > NS_SMALL_JOBS ? count : 0));
+    NsJob* jobs = many.empty() ? a.jobs : many.data();
+    int q = 1;
+    for (int k = 0; k < count; ++k) {
+        ns_job(mats[k], scale_rule, jobs[k]);
+        if (!jobs[k].vec) q = std::max(q, std::max(jobs[k].m, jobs[k].n));
+    }
+    if (!many.empty()) {
+        static_assert(sizeof(NsJob) % 4 == 0, "whole words");
+        const int rc = ns_upload(what, (const unsigned*)many.data(), many.size() * sizeof(NsJob) / 4, (unsigned*)g.ws, st);
+        if (rc) return rc;
+        a.table = (const NsJob*)g.ws;
+    }
+    const int lds = (int)sizeof(NsSmallLds);
 #define NS_SMALL_LAUNCH(NB)                                                                                          \
     do {                                                                                                             \
         opt[NB - 1].ensure((const void*)ns_small_kernel<T, MUON, NB>, lds);                                          \
-        hipLaunchKernelGGL((ns_small_kernel<T, MUON, NB>), dim3(some), dim3(512), lds, st, a);                       \
+        hipLaunchKernelGGL((ns_small_kernel<T, MUON, NB>), dim3(count), dim3(512), lds, st, a);                      \
     } while (0)
-        if (q <= 256) NS_SMALL_LAUNCH(1);
-        else if (q <= 512) NS_SMALL_LAUNCH(2);
-        else NS_SMALL_LAUNCH(3);
+    if (q <= 256) NS_SMALL_LAUNCH(1);
+    else if (q <= 512) NS_SMALL_LAUNCH(2);
+    else NS_SMALL_LAUNCH(3);
 #undef NS_SMALL_LAUNCH
-        DVAE_CHECK_LAUNCH(what);
-    }
+    DVAE_CHECK_LAUNCH(what);
     return DVAE_OK;
 }
 
@@ -348,14 +368,11 @@ int ns_plan(const char* what, const dvae_matrix* mats, int count, int scale_rule
 
 template <typename T, bool MUON>
 int ns_run(const char* what, const NsPlan& p, NsArgs g, int steps, hipStream_t st) {
-    // the table, as many kernel arguments at a time as fit
-    NsBlob blob;
-    if (p.njobs == 1) memcpy(&g.one, p.table.data() + (size_t)NS_PHASES * p.jp, sizeof(NsJob));
-    else for (size_t at = 0; at < p.table.size(); at += NsBlob::WORDS) {
-        const size_t n = p.table.size() - at < (size_t)NsBlob::WORDS ? p.table.size() - at : (size_t)NsBlob::WORDS;
-        memcpy(blob.w, p.table.data() + at, n * 4);
-        hipLaunchKernelGGL(ns_table_kernel, dim3(1), dim3(256), 0, st, blob, (unsigned*)g.ws + at, (int)n);
-        DVAE_CHECK_LAUNCH(what);
+    if (p.njobs == 1) {
+        memcpy(&g.one, p.table.data() + (size_t)NS_PHASES * p.jp, sizeof(NsJob));
+    } else {
+        const int rc = ns_upload(what, p.table.data(), p.table.size(), (unsigned*)g.ws, st);
+        if (rc) return rc;
     }
     g.first = (const int*)g.ws;
     g.jobs = (const NsJob*)(g.ws + (size_t)NS_PHASES * p.jp * 4);
@@ -499,7 +516,7 @@ size_t dvae_newton_schulz_workspace_bytes(const dvae_matrix* mats, int count) {
         for (int i = 0; i < count; ++i)
             if (mats[i].rows <= 0 || mats[i].cols <= 0 || mats[i].rows > (1 << 30) || mats[i].cols > (1 << 30) ||
                 mats[i].rows * mats[i].cols >= (1LL << 31)) return 0;
-        if (ns_all_small(mats, count)) return 256;        // not used; the least there is
+        if (ns_all_small(mats, count)) return ns_small_bytes(count);
         NsPlan p;
         return ns_plan("newton_schulz", mats, count, DVAE_MUON_SPECTRAL, p) ? 0 : p.bytes;
     } catch (...) {
@@ -521,7 +538,7 @@ int dvae_newton_schulz(const dvae_matrix* mats, int count, const double* coeffic
         g.a = (float)coefficients[0]; g.b = (float)coefficients[1]; g.c = (float)coefficients[2];
         g.eps = eps;
         const bool small = ns_all_small(mats, count);
-        if (small && (rc = ns_workspace_check("newton_schulz", workspace, workspace_bytes, 256))) return rc;
+        if (small && (rc = ns_workspace_check("newton_schulz", workspace, workspace_bytes, ns_small_bytes(count)))) return rc;
         if (small)
             return dtype == DVAE_F32 ? ns_run_small<float, false>("newton_schulz", mats, count, DVAE_MUON_SPECTRAL, g, steps, S(st))
                                      : ns_run_small<bf16, false>("newton_schulz", mats, count, DVAE_MUON_SPECTRAL, g, steps, S(st));
@@ -552,7 +569,7 @@ int dvae_muon_step(const dvae_matrix* mats, int count, double lr, double momentu
         g.mu = (float)momentum; g.nu = (float)(1.0 - momentum); g.nesterov = nesterov; g.lr = (float)lr;
         g.decay = (float)(1.0 - lr * weight_decay);
         if (ns_all_small(mats, count)) {
-            if ((rc = ns_workspace_check("muon_step", workspace, workspace_bytes, 256))) return rc;
+            if ((rc = ns_workspace_check("muon_step", workspace, workspace_bytes, ns_small_bytes(count)))) return rc;
             return ns_run_small<float, true>("muon_step", mats, count, scale_rule, g, steps, S(st));
         }
         NsPlan p;

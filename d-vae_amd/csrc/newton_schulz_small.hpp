@@ -20,6 +20,7 @@ constexpr int NS_SMALL_P = 64, NS_SMALL_Q = 768, NS_SMALL_VEC = 1 << 15, NS_SMAL
 
 struct NsSmallArgs {
     NsJob jobs[NS_SMALL_JOBS];
+    const NsJob* table;                                   // on the device, where there are more: then not NULL
     double eps;
     float a, b, c;
     float mu, nu, lr, decay;
@@ -48,7 +49,7 @@ template <typename T, bool MUON, int NB>
 __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
     extern __shared__ __align__(16) char smem[];
     NsSmallLds& s = *reinterpret_cast<NsSmallLds*>(smem);
-    const NsJob& j = g.jobs[blockIdx.x];
+    const NsJob j = g.table ? g.table[blockIdx.x] : g.jobs[blockIdx.x];
     const int m = j.m, n = j.n;
     const long xs = j.xs, os = j.os;
     const auto x = as_global<const T>(j.x);

@@ -56,6 +56,8 @@ def _forward(x, weight, bias, eps, save):
 def _backward(ctx, dy):
     x, weight, stats = ctx.saved_tensors
     want_x, want_w, want_b, _ = ctx.needs_input_grad
+    if dy.dtype != x.dtype:
+        dy = dy.to(x.dtype)
     with L.on_device(x.device):
         c = x.shape[-1]
         x2, dy2 = _rows(x, c), _rows(dy, c)

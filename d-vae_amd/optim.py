@@ -32,7 +32,7 @@ def newton_schulz(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     (a, b, c) = ``coefficients``, which drives every singular value towards 1 and leaves the singular vectors.
 
     ``x``: a float32 or bfloat16 device tensor of shape [..., m, n], or a list of them of one type (any shapes: the whole list
-    is one batch of launches).  Returns the same, in x's type.  The products have float32 accuracy for either type.  The
+    is one batch of launches, 65536 matrices at most).  Returns the same, in x's type and layout.  The products have float32 accuracy for either type.  The
     result is not differentiable."""
     many = isinstance(x, (list, tuple))
     xs = list(x) if many else [x]
@@ -126,7 +126,7 @@ def muon_step(params, grads, momenta, lr=0.02, momentum=0.95, nesterov=True, wei
         coef = array("d", coefficients)
         if len(coef) != 3:
             raise RuntimeError(f"muon_step: three coefficients, got {len(coef)}")
-        L.check(L.lib().dvae_muon_step(at, count, lr, momentum, int(nesterov), weight_decay, _SCALES[scale],
+        L.check(L.lib().dvae_muon_step(at, count, float(lr), float(momentum), int(nesterov), float(weight_decay), _SCALES[scale],
                                        coef.buffer_info()[0], int(steps), float(eps), ws.data_ptr(), size, L.stream()))
     torch.autograd.graph.increment_version([*params, *momenta])     # packed weights and saved tensors notice the step
 
@@ -135,6 +135,8 @@ class FusedMuon(torch.optim.Optimizer):
     """Muon over ``muon_step``: a torch optimiser (schedulers, param groups, ``state_dict``) for float32 device parameters.
     Parameters without a gradient are skipped.  Groups may differ in any option; each group is one batch of launches.  A step
     captured into a graph keeps the options it was captured with."""
+
+    _OPTIONS = ("lr", "momentum", "nesterov", "weight_decay", "steps", "coefficients", "eps", "scale")
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=COEFFICIENTS,
                  eps=1e-7, scale="spectral"):
@@ -161,12 +163,8 @@ class FusedMuon(torch.optim.Optimizer):
                 if "momentum_buffer" not in state:
                     state["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
                 momenta.append(state["momentum_buffer"])
-            muon_step(params, [p.grad.contiguous() for p in params], momenta,
-                      **{k: v for k, v in group.items() if k in self.defaults and k in _STEP_OPTIONS})
+            muon_step(params, [p.grad.contiguous() for p in params], momenta, **{k: group[k] for k in self._OPTIONS})
         return loss
-
-
-_STEP_OPTIONS = ("lr", "momentum", "nesterov", "weight_decay", "steps", "coefficients", "eps", "scale")
 
 
 class FusedAdam(torch.optim.Optimizer):

@@ -117,6 +117,36 @@ def test_other_layouts():
     held(leaf.grad, dx, ln_grad_bounds(x, ones, dx, xh, inv, w, 48, 60)[0])
 
 
+def test_offsets_past_32_bits():
+    """Rows 2^26 elements apart: the last ones start beyond 2^31 elements and 2^32 bytes."""
+    rows, c, apart = 36, 200, 1 << 26
+    x, dy, w, b = make(rows, c, torch.bfloat16)
+    big = torch.empty(rows * apart, dtype=torch.bfloat16, device="cuda")
+    xin = big.as_strided((rows, c), (apart, 1))
+    dyin = big.as_strided((rows, c), (apart, 1), 1 << 20)
+    xin.copy_(x)
+    dyin.copy_(dy)
+    check(x, dy, w, b, xin=xin, dyin=dyin)
+    lib = L.lib()
+    leaf = x.clone().requires_grad_(True)
+    want = dvae_amd.layer_norm(leaf, w, b)
+    out = big.as_strided((rows, c), (apart, 1), 2 << 20)
+    L.check(lib.dvae_layer_norm_fwd(xin.data_ptr(), apart, w.data_ptr(), b.data_ptr(), out.data_ptr(), apart, None, None, rows, c, 1e-5,
+                                    L.BF16, L.stream()))
+    assert torch.equal(out, want)
+
+
+def test_strided_parameters_and_another_gradient_type():
+    x, dy, w, b = make(33, 72, torch.bfloat16)
+    wide = torch.stack([w, b], 1).contiguous()
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    ref = torch.autograd.grad(dvae_amd.layer_norm(*leaves), leaves, dy)
+    wide.requires_grad_(True)
+    y = dvae_amd.layer_norm(leaves[0], wide[:, 0], wide[:, 1])
+    g, = torch.autograd.grad(y, wide, dy.float())
+    assert torch.equal(g[:, 0], ref[1]) and torch.equal(g[:, 1], ref[2])
+
+
 def test_gradients_of_some_inputs_only():
     x, dy, w, b = make(33, 72, torch.bfloat16)
     full = [t.clone().requires_grad_(True) for t in (x, w, b)]

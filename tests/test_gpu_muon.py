@@ -77,6 +77,16 @@ def test_list_of_any_shapes_is_each_alone():
         held(y, x)
 
 
+@pytest.mark.parametrize("m,n,batch", [(16, 24, 33), (64, 64, 300), (9, 700, 40)])
+def test_many_small_matrices(m, n, batch):
+    g = torch.Generator().manual_seed(m)
+    x = torch.randn(batch, m, n, generator=g).cuda()
+    y = dvae_amd.newton_schulz(x)
+    for i in {0, 1, 31, 32, batch // 2, batch - 1}:
+        held(y[i], x[i])
+        assert torch.equal(dvae_amd.newton_schulz(x[i]), y[i])
+
+
 def test_batches_and_layouts():
     x = torch.stack([matrix(40, 72, seed=i) for i in range(6)])
     y = dvae_amd.newton_schulz(x)
@@ -268,6 +278,49 @@ def test_classifier_trains_by_it():
         out = model(x)
         model._engine.invalidate()
         assert torch.equal(out, model(x)) and bool(out.isfinite().all())
+
+
+def test_dvae_trains_by_it():
+    """The D-VAE's trainer with the optimiser a config names: parameters off the hot path have no gradient and stay."""
+    torch.manual_seed(0)
+    from dvae_amd import data as DD
+    ds = DD.synthetic_cifar(n=128, seed=2)
+    loaders = DD.DatasetGenerator(ds, train_batch_size=64, device="cuda").getDataLoader(train_shuffle=True, train_drop_last=True)
+    model = dvae_amd.ResNet18DVAE(num_classes=10, stem_end_block=7, latent_dim=256)
+    model.spatial_emb = True
+    model.set_spatial_emb()
+    model = model.cuda()
+    opt = CFG.from_dict({"optimizer": {"name": "FusedMuon", "lr": 0.01}}).optimizer(model.parameters())
+
+    class Cfg:
+        grad_clip, log_frequency = 5.0, 100
+    trainer = dvae_amd.VAE_Trainer(loaders, None, Cfg(), stage=0)
+    model.train()
+    off = model.layer3[0].conv1.weight.detach().clone()
+    for images, labels in loaders["train_dataset"]:
+        before = {n: p.detach().clone() for n, p in model.named_parameters()}
+        old = {n: opt.state[p].get("momentum_buffer", torch.zeros_like(p)).clone() for n, p in model.named_parameters()}
+        payload = trainer.train_batch(images, labels, model, None, opt, 0)
+        assert math.isfinite(payload["loss"])
+        for n, p in model.named_parameters():
+            if n in ("conv1.weight", "decoder1.0.weight", "fc_mu.weight", "bn1.bias"):
+                want, _, tol, _ = muon_expected(before[n], p.grad, old[n], lr=0.01)
+                assert float((p.detach().double().cpu() - want).norm()) <= tol, n
+    assert torch.equal(off, model.layer3[0].conv1.weight.detach())
+
+
+def test_offsets_past_32_bits():
+    """Rows 2^27 elements apart."""
+    x = matrix(40, 60, seed=1)
+    big = torch.empty(40 << 27, dtype=torch.float32, device="cuda")
+    v = big.as_strided((40, 60), (1 << 27, 1))
+    v.copy_(x)
+    assert torch.equal(dvae_amd.newton_schulz(v), dvae_amd.newton_schulz(x))
+    y = matrix(66, 70, seed=2)                                  # through the batched kernels
+    big = big[:(34 << 27)].view(-1)
+    v = big.as_strided((66, 70), (1 << 26, 1))
+    v.copy_(y)
+    assert torch.equal(dvae_amd.newton_schulz(v), dvae_amd.newton_schulz(y))
 
 
 def test_side_stream_and_captured_step():
