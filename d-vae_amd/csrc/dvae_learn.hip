@@ -397,20 +397,20 @@ int ns_run(const char* what, const NsPlan& p, NsArgs g, int steps, hipStream_t s
     NS_LAUNCH(NS_SPLIT, ns_split_kernel<T, MUON>);
     for (int k = 0; k < steps; ++k) {
         if (p.gram_ts == 64) {
-            if (!p.gram_pieces) NS_LAUNCH_TILES(NS_GRAM, 64, 1, ns_symmetric_kernel<64, false, false, 1>);
+            if (!p.gram_pieces) NS_LAUNCH_TILES(NS_GRAM, 64, 1, ns_symmetric_kernel<64, false, false>);
             else {
-                NS_LAUNCH_TILES(NS_GRAM, 64, 1, ns_symmetric_kernel<64, false, true, 1>);
+                NS_LAUNCH_TILES(NS_GRAM, 64, 1, ns_symmetric_kernel<64, false, true>);
                 NS_LAUNCH_N(p.total[NS_GRAM_TILES] * 4, 1, 0, ns_gram_sum_kernel<64>);
             }
         } else if (!p.gram_pieces) {
-            NS_LAUNCH_TILES(NS_GRAM, 128, 1, ns_symmetric_kernel<128, false, false, 1>);
+            NS_LAUNCH_TILES(NS_GRAM, 128, 1, ns_symmetric_kernel<128, false, false>);
         } else {
-            NS_LAUNCH_TILES(NS_GRAM, 128, 1, ns_symmetric_kernel<128, false, true, 1>);
+            NS_LAUNCH_TILES(NS_GRAM, 128, 1, ns_symmetric_kernel<128, false, true>);
             NS_LAUNCH_N(p.total[NS_GRAM_TILES] * 16, 1, 0, ns_gram_sum_kernel<128>);
         }
         if (p.square_ts == 32) NS_LAUNCH(NS_SQUARE, ns_square_small_kernel);
-        else if (p.square_ts == 64) NS_LAUNCH_TILES(NS_SQUARE, 64, 1, ns_symmetric_kernel<64, true, false, 1>);
-        else NS_LAUNCH_TILES(NS_SQUARE, 128, 1, ns_symmetric_kernel<128, true, false, 1>);
+        else if (p.square_ts == 64) NS_LAUNCH_TILES(NS_SQUARE, 64, 1, ns_symmetric_kernel<64, true, false>);
+        else NS_LAUNCH_TILES(NS_SQUARE, 128, 1, ns_symmetric_kernel<128, true, false>);
         const bool last = k + 1 == steps;
         if (p.apply_ts == 128 && p.apply_groups == 1) {
             if (last) NS_LAUNCH_TILES(NS_APPLY, 128, 1, ns_last_kernel<128, T, MUON, 1>);

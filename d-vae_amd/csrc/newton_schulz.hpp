@@ -266,7 +266,7 @@ __device__ inline void ns_wave_sync() {
 // ---- the products ----------------------------------------------------------------------------------------------------
 // C[i][k] = sum over c of L[i][c] R[k][c] for a TS x TS tile: four waves, a quarter tile each, 32x32x16 MFMAs.  Two LDS
 // stages of one line (32 columns) per row, one barrier a line: while one half of a line is multiplied, the fragments of the
-// other half are on their way from LDS, and the next lines are on their way from memory in sets of registers.
+// other half are on their way from LDS, and the next two lines are on their way from memory in two sets of registers.
 // A line's eight 16-byte chunks are stored at chunk ^ (row / 2 & 7): of a fragment's rows any sixteen that are read at a time
 // meet the 64 banks once each.
 //
@@ -278,10 +278,7 @@ struct NsTile {
     static constexpr int PASS = TS / 32;                 // passes of 256 threads over a stage of one operand
     static constexpr int STAGES = 2 * 2 * TS * 128;      // bytes of a group
     static constexpr int BYTES = G * STAGES;
-    static constexpr int AHEAD = 2;                      // lines on their way from memory
     f32x16 acc[S][S];
-    // A dependent MFMA waits for two times its issue: a wave with a single subtile sums its three products apart.
-    f32x16 side[2];
     int from = 0, to = S;                                // rows of subtiles that are this group's after join
 
     struct Lines { u32x4 l[PASS], r[PASS]; };
@@ -294,7 +291,6 @@ struct NsTile {
             for (int k = 0; k < S; ++k)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[i][k][e] = 0.f;
-        side[0] = side[1] = acc[0][0];
     }
 
     // MFMAs FROM to TO of the 3 S^2 of half a line
@@ -303,8 +299,7 @@ struct NsTile {
 #pragma unroll
         for (int m = FROM; m < TO; ++m) {
             const int w = m / (S * S), i = m / S % S, n = m % S;
-            f32x16& to = S == 1 && w < 2 ? side[w] : acc[i][n];
-            to = __builtin_amdgcn_mfma_f32_32x32x16_f16(w == 1 ? f.ll[i] : f.lh[i], w == 0 ? f.rl[n] : f.rh[n], to, 0, 0, 0);
+            acc[i][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w == 1 ? f.ll[i] : f.lh[i], w == 0 ? f.rl[n] : f.rh[n], acc[i][n], 0, 0, 0);
         }
     }
     // `lines` is even; rows past lrows / rrows re-read the last one: their results are not stored
@@ -328,7 +323,7 @@ struct NsTile {
             lp[i] = L + (((long)line0 * 8 + chunk) * lrows + min(l0 + i * 32 + row, lrows - 1)) * 16;
             rp[i] = R + (((long)line0 * 8 + chunk) * rrows + min(r0 + i * 32 + row, rrows - 1)) * 16;
         }
-        Lines set[AHEAD];
+        Lines set[2];
         int ahead = lines;
         auto fetch = [&](Lines& s) {                      // the next line; past the last one, that one again
 #pragma unroll
@@ -369,28 +364,26 @@ struct NsTile {
             }
         };
         Frags f0, f1;
-#pragma unroll
-        for (int d = 0; d < AHEAD; ++d) fetch(set[d]);
+        fetch(set[0]);
+        fetch(set[1]);
         stage(0, set[0]);
         fetch(set[0]);
         __syncthreads();
         read(f0, 0, 0);
-        for (int k = 0; k < lines; k += AHEAD) {
+        for (int k = 0; k < lines; k += 2) {
 #pragma unroll
-            for (int d = 0; d < AHEAD; ++d) {
-                const int next = (d + 1) % AHEAD;
-                read(f1, d & 1, 1);
+            for (int d = 0; d < 2; ++d) {
+                read(f1, d, 1);
                 multiply<0, S * S>(f0);
-                stage((d & 1) ^ 1, set[next]);
+                stage(d ^ 1, set[d ^ 1]);
                 multiply<S * S, 3 * S * S>(f0);
-                fetch(set[next]);
+                fetch(set[d ^ 1]);
                 multiply<0, S * S>(f1);
                 __syncthreads();                          // this line's fragments are out, the next line is in
-                read(f0, (d & 1) ^ 1, 0);
+                read(f0, d ^ 1, 0);
                 multiply<S * S, 3 * S * S>(f1);
             }
         }
-        if (S == 1) acc[0][0] += side[0] + side[1];
     }
 
     // Adds the groups up: each keeps a row of subtiles.
@@ -480,17 +473,17 @@ __device__ inline void ns_triangle(int t, int& i, int& k) {
 
 // The symmetric products store the tiles at and below the diagonal and their mirror images.  Tiles on the diagonal are
 // stored once: their two halves agree to rounding only, and two writers of one place would leave either's.
-template <int TS, int G>
-__device__ inline void ns_store_symmetric(NsTile<TS, G>& c, char* smem, gbytes dst, int P, int ti, int tk) {
+template <int TS>
+__device__ inline void ns_store_symmetric(NsTile<TS>& c, char* smem, gbytes dst, int P, int ti, int tk) {
     constexpr int S = NsTile<TS>::S;
-    const int wave = threadIdx.x >> 6, wr = (wave >> 1 & 1) * (TS / 2), wc = (wave & 1) * (TS / 2);
+    const int wave = threadIdx.x >> 6, wr = (wave >> 1) * (TS / 2), wc = (wave & 1) * (TS / 2);
     unsigned* patch = reinterpret_cast<unsigned*>(smem) + wave * (32 * 36);
 #pragma unroll
     for (int i = 0; i < S; ++i)
 #pragma unroll
         for (int k = 0; k < S; ++k) {
             const int row = ti * TS + wr + i * 32, col = tk * TS + wc + k * 32;
-            if (row >= P || col >= P || i < c.from || i >= c.to) continue;
+            if (row >= P || col >= P) continue;
             ns_store(c.acc[i][k], patch, ns_line(dst, P, row, col), P, ti != tk ? ns_line(dst, P, col, row) : gbytes(nullptr), P);
         }
 }
@@ -525,8 +518,8 @@ __device__ inline void ns_symmetric_value(const NsArgs& g, const NsPlanes& w, f3
 // The symmetric products, tiles at and below the diagonal: whole or (Gram, where the tiles alone would leave much of the chip
 // idle) in pieces of the contraction, a job's kc lines each, that leave fp32 partial tiles for ns_gram_sum_kernel.  Neighbouring
 // workgroups take different tiles of the same lines: an XCD reads a part of X once.
-template <int TS, bool SQUARE, bool PIECES, int G>
-__global__ __launch_bounds__(256 * G, G == 1 ? 2 : 1) void ns_symmetric_kernel(NsArgs g) {
+template <int TS, bool SQUARE, bool PIECES>
+__global__ __launch_bounds__(256, 2) void ns_symmetric_kernel(NsArgs g) {
     extern __shared__ __align__(16) char smem[];
     constexpr int S = NsTile<TS>::S;
     int t, ti, tk;
@@ -536,11 +529,10 @@ __global__ __launch_bounds__(256 * G, G == 1 ? 2 : 1) void ns_symmetric_kernel(N
     const int side = (w.P + TS - 1) / TS, tiles = side * (side + 1) / 2;
     const int lines = (SQUARE ? w.P : w.Q) / 32, kc = j.kc, line0 = PIECES ? t / tiles * kc : 0;
     ns_triangle(PIECES ? t % tiles : t, ti, tk);
-    NsTile<TS, G> c;
+    NsTile<TS> c;
     c.zero();
     const cgbytes m = SQUARE ? w.a : w.x;
     c.run(m, w.P, ti * TS, m, w.P, tk * TS, line0, PIECES ? min(kc, lines - line0) : lines, smem);
-    c.join(smem);
     if (PIECES) {
         const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
         const auto out = as_global<float>(g.part) + (long)wg * (TS * TS) + lane * 4;
@@ -561,7 +553,7 @@ __global__ __launch_bounds__(256 * G, G == 1 ? 2 : 1) void ns_symmetric_kernel(N
 #pragma unroll
         for (int k = 0; k < S; ++k) {
             const int row = ti * TS + NsTile<TS>::row_of(i, 0), col = tk * TS + NsTile<TS>::col_of(k);
-            if (row < w.P && col < w.P && i >= c.from && i < c.to) ns_symmetric_value<SQUARE>(g, w, c.acc[i][k], row, col);
+            if (row < w.P && col < w.P) ns_symmetric_value<SQUARE>(g, w, c.acc[i][k], row, col);
         }
     ns_store_symmetric(c, smem, SQUARE ? w.b : w.a, w.P, ti, tk);
 }
@@ -617,8 +609,8 @@ __global__ __launch_bounds__(256) void ns_gram_sum_kernel(NsArgs g) {
 
 // B = a I + b A + c A^2 for matrices whose A is small against the chip: tiles of 32, a workgroup each, so that many CUs fetch; its
 // four waves take every fourth line and feed their MFMAs straight from memory (a tile's rows are read once a workgroup: LDS would
-// only add its latency and a barrier a line).  What is left is a chain of four latencies: 36 tiles of 64 take 8.2 us for p = 512,
-// 136 of these %D512%.
+// only add its latency and a barrier a line).  What is left is a chain of latencies (arguments, loads, exchange, store): for
+// p = 512, 36 staged tiles of 64 take 8.9 us, 136 of these 6.5 us; for p = 64 it is 4.5 and 3.6.
 __global__ __launch_bounds__(256, 2) void ns_square_small_kernel(NsArgs g) {
     __shared__ f32x4 red[4][4][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;

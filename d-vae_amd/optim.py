@@ -96,13 +96,16 @@ def muon_step(params, grads, momenta, lr=0.02, momentum=0.95, nesterov=True, wei
     if scale not in _SCALES:
         raise RuntimeError(f"muon_step: scale {scale!r} ({sorted(_SCALES)})")
     table, written, read = array("q"), set(), set()
-    device = params[0].device if params else None
+    device, f32 = params[0].device if params else None, torch.float32
+    if device is not None and device.type != "cuda":
+        raise RuntimeError("muon_step runs on libdvae_hip: it takes device tensors")
     for i, (p, g, m) in enumerate(zip(params, grads, momenta)):
         shape = p.shape
-        for what, t in (("parameter", p), ("gradient", g), ("momentum", m)):
-            if t.dtype != torch.float32 or not t.is_cuda or t.device != device or t.shape != shape or not t.is_contiguous():
-                raise RuntimeError(f"muon_step: {what} {i} must be a contiguous float32 tensor of shape {tuple(shape)} on one "
-                                   f"device, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        if not (p.dtype == f32 and g.dtype == f32 and m.dtype == f32 and g.shape == shape and m.shape == shape and
+                p.device == device and g.device == device and m.device == device and
+                p.is_contiguous() and g.is_contiguous() and m.is_contiguous()):
+            raise RuntimeError(f"muon_step: parameter, gradient and momentum {i} must be contiguous float32 tensors of one shape on "
+                               f"{device}, got " + ", ".join(f"{t.dtype} {tuple(t.shape)} {t.stride()} on {t.device}" for t in (p, g, m)))
         n = p.numel()
         if n == 0:
             continue
