@@ -31,12 +31,13 @@ def _check(x, weight, bias, eps):
 
 def _rows(t, c):
     """t as rows of c adjacent elements: a view wherever strides allow it (padded, sliced and expanded rows do)."""
-    t = t.reshape(-1, c)
+    if t.dim() != 2:
+        t = t.reshape(-1, c)
     return t if t.stride(1) == 1 or c == 1 else t.contiguous()
 
 
 def _param(p):
-    return None if p is None else p.contiguous()
+    return p if p is None or p.is_contiguous() else p.contiguous()
 
 
 def _forward(x, weight, bias, eps, save):
