@@ -272,7 +272,7 @@ int ns_plan(const char* what, const dvae_matrix* mats, int count, int scale_rule
     // Tile sizes by the work they make, in us of a CU: a line of a 128-tile costs it 0.78, of a 64-tile 0.28 (measured with the chip
     // full; a 128-tile is four of those), and a tile's start and end about 3 and 1.2.  Padding decides: 64-row matrices want 64.
     double cost[3][2] = {};                               // Gram, square, apply; tiles of 64, of 128
-    long longest[2] = {1, 1}, lines[2] = {}, tiles[3][2] = {}, tiles32 = 0;
+    long longest[2] = {1, 1}, lines[2] = {}, tiles[3][2] = {}, tiles32 = 0, lines32 = 0;
     for (int i = 0; i < count; ++i) {
         const dvae_matrix& m = mats[i];
         if (m.vector) continue;
@@ -290,6 +290,7 @@ int ns_plan(const char* what, const dvae_matrix* mats, int count, int scale_rule
             tiles[2][big] += (long)((P + ts - 1) / ts) * ((Q + ts - 1) / ts);
         }
         tiles32 += ns_triangles(P, 32);
+        lines32 += ns_triangles(P, 32) * (Q / 32);
         longest[0] = longest[0] > Q / 32 ? longest[0] : Q / 32;
         longest[1] = longest[1] > P / 32 ? longest[1] : P / 32;
         p.matrices = true;
@@ -303,6 +304,26 @@ int ns_plan(const char* what, const dvae_matrix* mats, int count, int scale_rule
     // (2048 x 2048: 53 us whole in tiles of 64, 45 + 12 us in pieces of tiles of 128).
     const bool cut_gram = tiles[0][0] < 512;
     if (!cut_gram && tiles[0][1] < 512) p.gram_ts = 64;
+    // Straight from memory in tiles of 32 where that is sooner done.  Times in us, measured: the pieces and their sum have 13 beside
+    // their work (512 x 4608: 17 us in all, the D-VAE's matrices 16); a workgroup of the other 0.12 a line and 3, another 5 where it
+    // leaves pieces (144 lines: 20 us; the D-VAE's: 12 us).
+    const long direct_kc = lines32 / 256 > 32 ? lines32 / 256 : 32;
+    auto direct_piece = [&](long all) {                   // lines of a workgroup: a CU's share of all, in equal pieces
+        const long n = all / direct_kc > 1 ? all / direct_kc : 1;
+        return (int)((all + n - 1) / n);
+    };
+    if (cut_gram) {
+        int longest_piece = 0;
+        bool several = false;
+        for (int i = 0; i < count; ++i) {
+            if (mats[i].vector) continue;
+            const int all = ns_pad((int)(mats[i].rows < mats[i].cols ? mats[i].cols : mats[i].rows)) / 32, piece = direct_piece(all);
+            longest_piece = std::max(longest_piece, piece);
+            several = several || piece < all;
+        }
+        const double direct = fmax(longest_piece * 0.12, lines32 * 0.1 / 256) + (several ? 8.0 : 3.0);
+        if (direct < cost[0][p.gram_ts == 128] / 256 + 13.0) p.gram_ts = 32;
+    }
     const int gb = p.gram_ts == 128;
     const int gram_kc = (int)((lines[gb] + 511) / 512);
     // The square has p / 32 lines and few tiles: straight from memory in tiles of 32 up to about two workgroups of those a SIMD
@@ -340,7 +361,7 @@ int ns_plan(const char* what, const dvae_matrix* mats, int count, int scale_rule
         const int P = ns_pad(j.m < j.n ? j.m : j.n), Q = ns_pad(j.m < j.n ? j.n : j.m);
         off += ns_job_bytes(j.m, j.n);
         p.total[NS_SPLIT] += (long)(P / 64) * (Q / 64);
-        j.kc = piece(cut_gram, gram_kc, Q / 32);
+        j.kc = p.gram_ts == 32 ? direct_piece(Q / 32) : piece(cut_gram, gram_kc, Q / 32);
         const long gp = (Q / 32 + j.kc - 1) / j.kc;
         if (gp > 1) p.gram_pieces = true;
         p.total[NS_GRAM] += ns_triangles(P, p.gram_ts) * gp;
@@ -396,7 +417,10 @@ int ns_run(const char* what, const NsPlan& p, NsArgs g, int steps, hipStream_t s
     if (!p.matrices) return DVAE_OK;
     NS_LAUNCH(NS_SPLIT, ns_split_kernel<T, MUON>);
     for (int k = 0; k < steps; ++k) {
-        if (p.gram_ts == 64) {
+        if (p.gram_ts == 32) {
+            NS_LAUNCH_N(p.total[NS_GRAM], 2, 0, ns_direct_kernel<false, 8>);
+            if (p.gram_pieces) NS_LAUNCH(NS_GRAM_TILES, ns_direct_sum_kernel);
+        } else if (p.gram_ts == 64) {
             if (!p.gram_pieces) NS_LAUNCH_TILES(NS_GRAM, 64, 1, ns_symmetric_kernel<64, false, false>);
             else {
                 NS_LAUNCH_TILES(NS_GRAM, 64, 1, ns_symmetric_kernel<64, false, true>);
@@ -408,7 +432,7 @@ int ns_run(const char* what, const NsPlan& p, NsArgs g, int steps, hipStream_t s
             NS_LAUNCH_TILES(NS_GRAM, 128, 1, ns_symmetric_kernel<128, false, true>);
             NS_LAUNCH_N(p.total[NS_GRAM_TILES] * 16, 1, 0, ns_gram_sum_kernel<128>);
         }
-        if (p.square_ts == 32) NS_LAUNCH(NS_SQUARE, ns_square_small_kernel);
+        if (p.square_ts == 32) NS_LAUNCH(NS_SQUARE, ns_direct_kernel<true, 4>);
         else if (p.square_ts == 64) NS_LAUNCH_TILES(NS_SQUARE, 64, 1, ns_symmetric_kernel<64, true, false>);
         else NS_LAUNCH_TILES(NS_SQUARE, 128, 1, ns_symmetric_kernel<128, true, false>);
         const bool last = k + 1 == steps;

@@ -607,42 +607,67 @@ __global__ __launch_bounds__(256) void ns_gram_sum_kernel(NsArgs g) {
     ns_store(a, patch, ns_line(w.a, w.P, row, col), w.P, ti != tk ? ns_line(w.a, w.P, col, row) : gbytes(nullptr), w.P);
 }
 
-// B = a I + b A + c A^2 for matrices whose A is small against the chip: tiles of 32, a workgroup each, so that many CUs fetch; its
-// four waves take every fourth line and feed their MFMAs straight from memory (a tile's rows are read once a workgroup: LDS would
-// only add its latency and a barrier a line).  What is left is a chain of latencies (arguments, loads, exchange, store): for
-// p = 512, 36 staged tiles of 64 take 8.9 us, 136 of these 6.5 us; for p = 64 it is 4.5 and 3.6.
-__global__ __launch_bounds__(256, 2) void ns_square_small_kernel(NsArgs g) {
-    __shared__ f32x4 red[4][4][64];
+// ---- symmetric products straight from memory -----------------------------------------------------------------------------
+// Where the tiles of a symmetric product are few, tiles of 32, a workgroup of W waves each: many CUs fetch, the waves take every
+// W-th line and feed their MFMAs from memory, four lines in flight (a tile's rows are read once a workgroup: LDS would only
+// add its latency and a barrier a line), and add up through LDS at the end, a quarter of the tile for each of four waves.  What is
+// left is a chain of latencies (arguments, loads, exchange, store) and, for long contractions, what the L2 gives a CU (35 B a
+// clock).  The square: for p = 512, 36 staged tiles of 64 take 8.9 us, 136 of these 6.5 us; for p = 64 4.5 and 3.6.  X X^T: the
+// D-VAE's matrices 7 + 5 us (with the sum of the longest one's pieces) against 8.5 + 7.5 us staged, 512 x 4608 20 against 17 us.
+
+// A quarter of a 32x32 tile at (ti, tk) of a symmetric operand, four rows of a lane's column, to both of its places.
+__device__ inline void ns_store_quarter(gbytes base, long rows, int ti, int tk, int quarter, const float (&v)[4]) {
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    const int row = ti * 32 + 8 * quarter + 4 * half, col = tk * 32 + (lane & 31);
+    unsigned u[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[e] = ns_split(v[e]);
+    const gbytes dst = ns_line(base, rows, col, ti * 32) + quarter * rows * 16 + half * 8;
+    *(DVAE_GLOBAL u32x2*)dst = u32x2{(u[0] & 0xffffu) | (u[1] << 16), (u[2] & 0xffffu) | (u[3] << 16)};
+    *(DVAE_GLOBAL u32x2*)(dst + rows * 64) = u32x2{(u[0] >> 16) | (u[1] & 0xffff0000u), (u[2] >> 16) | (u[3] & 0xffff0000u)};
+    if (ti == tk) return;                                 // the tile holds both places' elements
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const gbytes p = ns_line(base, rows, row + e, tk * 32) + (lane >> 3 & 3) * rows * 16 + (lane & 7) * 2;
+        *(DVAE_GLOBAL unsigned short*)p = (unsigned short)u[e];
+        *(DVAE_GLOBAL unsigned short*)(p + rows * 64) = (unsigned short)(u[e] >> 16);
+    }
+}
+
+// A = X X^T, in pieces of a job's kc lines (more than one leave fp32 partial tiles for ns_direct_sum_kernel), or
+// B = a I + b A + c A^2.
+template <bool SQUARE, int W>
+__global__ __launch_bounds__(64 * W) void ns_direct_kernel(NsArgs g) {
+    __shared__ f32x4 red[W][4][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     int t, ti, tk;
-    const NsJob j = ns_job_of(g, ns_find(g, NS_SQUARE, blockIdx.x, t));
+    const int wg = ns_swizzle(blockIdx.x, g.total);
+    const NsJob j = ns_job_of(g, ns_find(g, SQUARE ? NS_SQUARE : NS_GRAM, wg, t));
     const NsPlanes w(g, j);
-    ns_triangle(t, ti, tk);
-    const int lines = w.P / 32;
+    const int all = (SQUARE ? w.P : w.Q) / 32, kc = SQUARE ? all : j.kc, tiles = (w.P / 32) * (w.P / 32 + 1) / 2;
+    const int from = t / tiles * kc, to = min(from + kc, all);
+    ns_triangle(t % tiles, ti, tk);
     const long rows = w.P;
-    const cgbytes lp = ns_line(w.a, rows, ti * 32 + (lane & 31), 0) + half * rows * 16, rp = ns_line(w.a, rows, tk * 32 + (lane & 31), 0) + half * rows * 16;
+    const gbytes m = SQUARE ? w.a : w.x;
+    const cgbytes lp = ns_line(m, rows, ti * 32 + (lane & 31), 0) + half * rows * 16, rp = ns_line(m, rows, tk * 32 + (lane & 31), 0) + half * rows * 16;
     f32x16 acc[3];
 #pragma unroll
     for (int k = 0; k < 3; ++k)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[k][e] = 0.f;
-    // this wave's quarter of the tile at the end: rows row .. row + 3 of column col, that is of A's row col
-    const int row = ti * 32 + 8 * wave + 4 * half, col = tk * 32 + (lane & 31);
-    const cgbytes own = ns_line(w.a, rows, col, ti * 32) + wave * rows * 16 + half * 8;
-    u32x2 oh, ol;
-    for (int line = wave; line < lines; line += 16) {
+    for (int line = from + wave; line < to; line += 4 * W) {
         f16x8 l[4][4], r[4][4];                           // [line][two halves of h, then of l]; past the last line that one again, unused
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const long at = (min(line + 4 * u, lines - 1) * 8 + c * 2) * rows * 16;
+                const long at = (min(line + W * u, to - 1) * 8 + c * 2) * rows * 16;
                 l[u][c] = *(const DVAE_GLOBAL f16x8*)(lp + at);
                 r[u][c] = *(const DVAE_GLOBAL f16x8*)(rp + at);
             }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            if (line + 4 * u >= lines) break;
+            if (line + W * u >= to) break;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[u][k], r[u][2 + k], acc[0], 0, 0, 0);
@@ -651,8 +676,6 @@ __global__ __launch_bounds__(256, 2) void ns_square_small_kernel(NsArgs g) {
             }
         }
     }
-    oh = *(const DVAE_GLOBAL u32x2*)own;
-    ol = *(const DVAE_GLOBAL u32x2*)(own + rows * 64);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
         f32x4 v;
@@ -661,21 +684,53 @@ __global__ __launch_bounds__(256, 2) void ns_square_small_kernel(NsArgs g) {
         red[wave][q][lane] = v;
     }
     __syncthreads();
-    const f32x4 v = (red[0][wave][lane] + red[1][wave][lane]) + (red[2][wave][lane] + red[3][wave][lane]);
-    unsigned u[4];
+    if (wave >= 4) return;
+    f32x4 v = red[0][wave][lane];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) u[e] = ns_split(ns_polynomial(g, v[e], oh, ol, e, row + e == col));
-    const gbytes dst = ns_line(w.b, rows, col, ti * 32) + wave * rows * 16 + half * 8;
-    *(DVAE_GLOBAL u32x2*)dst = u32x2{(u[0] & 0xffffu) | (u[1] << 16), (u[2] & 0xffffu) | (u[3] << 16)};
-    *(DVAE_GLOBAL u32x2*)(dst + rows * 64) = u32x2{(u[0] >> 16) | (u[1] & 0xffff0000u), (u[2] >> 16) | (u[3] & 0xffff0000u)};
-    if (ti != tk) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const gbytes p = ns_line(w.b, rows, row + e, tk * 32) + (lane >> 3 & 3) * rows * 16 + (lane & 7) * 2;
-            *(DVAE_GLOBAL unsigned short*)p = (unsigned short)u[e];
-            *(DVAE_GLOBAL unsigned short*)(p + rows * 64) = (unsigned short)(u[e] >> 16);
-        }
+    for (int o = 1; o < W; ++o) v += red[o][wave][lane];
+    if (!SQUARE && kc < all) {
+        as_global<f32x4>(g.part)[((long)wg * 4 + wave) * 64 + lane] = v;
+        return;
     }
+    float f[4];
+    if (SQUARE) {
+        // A's elements of this quarter: rows row .. row + 3 of column col, that is of row col, A being symmetric
+        const int row = ti * 32 + 8 * wave + 4 * half, col = tk * 32 + (lane & 31);
+        const cgbytes own = ns_line(w.a, rows, col, ti * 32) + wave * rows * 16 + half * 8;
+        const u32x2 h = *(const DVAE_GLOBAL u32x2*)own, l = *(const DVAE_GLOBAL u32x2*)(own + rows * 64);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = ns_polynomial(g, v[e], h, l, e, row + e == col);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = v[e] * (NS_SA / (NS_SX * NS_SX));
+    }
+    ns_store_quarter(SQUARE ? w.b : w.a, rows, ti, tk, wave, f);
+}
+
+// Adds the pieces of the matrices that have several, a workgroup a tile, always in the same order.
+__global__ __launch_bounds__(256) void ns_direct_sum_kernel(NsArgs g) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int t, ti, tk;
+    const int jn = ns_find(g, NS_GRAM_TILES, blockIdx.x, t);
+    const NsJob j = ns_job_of(g, jn);
+    const NsPlanes w(g, j);
+    const int all = w.Q / 32, tiles = (w.P / 32) * (w.P / 32 + 1) / 2, pieces = (all + j.kc - 1) / j.kc;
+    if (pieces == 1) return;
+    ns_triangle(t, ti, tk);
+    const auto in = as_global<const f32x4>(g.part) + (((g.njobs == 1 ? 0L : (long)g.first[NS_GRAM * g.jp + jn]) + t) * 4 + wave) * 64 + lane;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < pieces; s += 8) {
+        f32x4 r[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) r[u] = in[(long)min(s + u, pieces - 1) * tiles * 256];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (s + u < pieces) v += r[u];
+    }
+    float f[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = v[e] * (NS_SA / (NS_SX * NS_SX));
+    ns_store_quarter(w.a, w.P, ti, tk, wave, f);
 }
 
 // X <- B X, left in both orientations
