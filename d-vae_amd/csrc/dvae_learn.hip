@@ -57,7 +57,7 @@ constexpr int LN_GRID = 2048;
 
 int ln_check(const char* what, int64_t rows, int C, int dtype) {
     if (dtype != DVAE_F32 && dtype != DVAE_BF16) DVAE_FAIL(DVAE_EDTYPE, "%s: unknown dtype %d", what, dtype);
-    if (rows < 0 || C <= 0 || C > (1 << 30)) DVAE_FAIL(DVAE_EINVAL, "%s: bad shape %lld x %d", what, (long long)rows, C);
+    if (rows < 0 || C <= 0 || C >= (1 << 30)) DVAE_FAIL(DVAE_EINVAL, "%s: bad shape %lld x %d", what, (long long)rows, C);
     return DVAE_OK;
 }
 // an operand: present, element-aligned, rows that do not overlap where they are written
@@ -129,6 +129,9 @@ void ln_launch(const LnArgs& a, const LnShape& s, bool bwd, int groups, hipStrea
 
 // ---- Newton-Schulz ----------------------------------------------------------------------------------------------------
 inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+// Workgroups of a launch: 2^32 threads at 512 each.  Matrices that would need more do not fit the memory.
+constexpr long NS_MOST = (1L << 23) - 1;
 
 struct NsPlan {
     std::vector<unsigned> table;      // prefix arrays, then jobs, as they lie on the device
@@ -351,7 +354,7 @@ int ns_plan(const char* what, const dvae_matrix* mats, int count, int scale_rule
         j.nchunk = (int)(chunks < 1024 ? chunks : 1024);
         j.part = (int)part;
         for (int f = 0; f < NS_PHASES; ++f) {
-            if (p.total[f] > INT_MAX / 2) DVAE_FAIL(DVAE_EINVAL, "%s: too much work for one call", what);
+            if (p.total[f] > NS_MOST) DVAE_FAIL(DVAE_EINVAL, "%s: too much work for one call", what);
             first[(size_t)f * p.jp + i] = (int)p.total[f];
         }
         p.total[NS_NORM] += j.nchunk;
@@ -370,7 +373,7 @@ int ns_plan(const char* what, const dvae_matrix* mats, int count, int scale_rule
         p.total[NS_APPLY] += (long)((P + p.apply_ts - 1) / p.apply_ts) * ((Q + p.apply_ts - 1) / p.apply_ts);
     }
     for (int f = 0; f < NS_PHASES; ++f)
-        if (p.total[f] > INT_MAX / 2) DVAE_FAIL(DVAE_EINVAL, "%s: too much work for one call", what);
+        if (p.total[f] > NS_MOST) DVAE_FAIL(DVAE_EINVAL, "%s: too much work for one call", what);
     // jobs without tiles in a phase share their first with the next one that has some; those after the last such are beyond it
     const size_t words = first.size() + jobs.size() * sizeof(NsJob) / 4;
     p.table.resize(words);
@@ -475,7 +478,7 @@ int ns_workspace_check(const char* what, const void* ws, size_t have, size_t nee
 extern "C" {
 
 size_t dvae_layer_norm_workspace_bytes(int64_t rows, int C, int dtype) {
-    if (rows < 0 || C <= 0 || (dtype != DVAE_F32 && dtype != DVAE_BF16)) return 0;
+    if (rows < 0 || C <= 0 || C >= (1 << 30) || (dtype != DVAE_F32 && dtype != DVAE_BF16)) return 0;
     return (size_t)ln_bwd_groups(rows, C, dtype) * 2 * C * sizeof(float);
 }
 

@@ -57,7 +57,7 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
     const auto mom = as_global<float>(j.mom);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
     if (MUON && j.vec) {
-        for (long e = threadIdx.x; e < n; e += 512) {
+        for (long e = threadIdx.x; e < (long)m * n; e += 512) {
             const float gr = (float)x[e], p = (float)out[e];
             const float mi = g.mu * mom[e] + g.nu * gr;
             mom[e] = mi;

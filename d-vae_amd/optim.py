@@ -32,8 +32,8 @@ def newton_schulz(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     (a, b, c) = ``coefficients``, which drives every singular value towards 1 and leaves the singular vectors.
 
     ``x``: a float32 or bfloat16 device tensor of shape [..., m, n], or a list of them of one type (any shapes: the whole list
-    is one batch of launches, 65536 matrices at most).  Returns the same, in x's type and layout.  The products have float32 accuracy for either type.  The
-    result is not differentiable."""
+    is one batch of launches, 65536 matrices at most).  Returns the same, in x's type and layout.  The products have float32
+    accuracy for either type.  The result is not differentiable."""
     many = isinstance(x, (list, tuple))
     xs = list(x) if many else [x]
     outs, table, keep = [], array("q"), []
@@ -90,7 +90,7 @@ def muon_step(params, grads, momenta, lr=0.02, momentum=0.95, nesterov=True, wei
 
     with every parameter of two or more dimensions taken as the matrix [shape[0], rest] and s = sqrt(max(1, rows / cols))
     (``scale="spectral"``) or 0.2 sqrt(max(rows, cols)) (``"rms"``: steps as long as Adam's).  Parameters of fewer dimensions
-    (gains, biases) move by lr u.  All parameters go through the same dozen and a half launches."""
+    (gains, biases) move by lr u.  All parameters go through the same two dozen launches."""
     if not len(params) == len(grads) == len(momenta):
         raise RuntimeError(f"muon_step: {len(params)} parameters, {len(grads)} gradients, {len(momenta)} momenta")
     if scale not in _SCALES:
@@ -137,7 +137,8 @@ def muon_step(params, grads, momenta, lr=0.02, momentum=0.95, nesterov=True, wei
 class FusedMuon(torch.optim.Optimizer):
     """Muon over ``muon_step``: a torch optimiser (schedulers, param groups, ``state_dict``) for float32 device parameters.
     Parameters without a gradient are skipped.  Groups may differ in any option; each group is one batch of launches.  A step
-    captured into a graph keeps the options it was captured with."""
+    captured into a graph keeps the options it was captured with, and its replays change the weights without their models'
+    knowledge: ``model._engine.invalidate()`` before such a model's next eager call, as after writes through ``param.data``."""
 
     _OPTIONS = ("lr", "momentum", "nesterov", "weight_decay", "steps", "coefficients", "eps", "scale")
 

@@ -303,8 +303,8 @@ int dvae_clip_adam(float* p, const float* g, float* m, float* v, int64_t n, floa
  * one input row).  Pointers need the alignment of one element only.  gamma, beta and their gradients are fp32 [C], each
  * NULL if absent.  save_mean / save_invstd (fp32 [rows], both or neither) are what the backward pass reads; inference
  * passes NULL.  dx, dgamma and dbeta may each be NULL.  The workspace (16-byte aligned) is needed only for dgamma / dbeta.
- * rows == 0 is allowed: the gradients of gamma and beta are then zero.  Bitwise reproducible; a row's results do not depend
- * on the other rows. */
+ * C < 2^30; rows == 0 is allowed: the gradients of gamma and beta are then zero.  Bitwise reproducible; a row's results do
+ * not depend on the other rows. */
 size_t dvae_layer_norm_workspace_bytes(int64_t rows, int C, int dtype);
 int dvae_layer_norm_fwd(const void* x, int64_t x_stride, const float* gamma, const float* beta, void* y, int64_t y_stride,
                         float* save_mean, float* save_invstd, int64_t rows, int C, float eps, int dtype, void* stream);

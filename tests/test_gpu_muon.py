@@ -185,6 +185,26 @@ def test_many_parameters():
     step_held([(40, 3, 3, 3), (40000,), (9,)], seed=6)
 
 
+@pytest.mark.parametrize("beside", [None, (80, 100)])      # alone in the one-launch kernel; among the batched phases
+def test_c_entry_steps_every_row_of_a_vector(beside):
+    import array
+    shapes = [(3, 50)] + ([beside] if beside else [])
+    p, g, m = params_of(shapes)
+    mu, lr = 0.9, 0.1
+    m64 = mu * m[0].double() + (1 - mu) * g[0].double()
+    p64 = p[0].double() - lr * ((1 - mu) * g[0].double() + mu * m64)
+    rows = [(g[i].data_ptr(), p[i].data_ptr(), m[i].data_ptr(), *s, s[1], s[1], int(i == 0)) for i, s in enumerate(shapes)]
+    table, coef, lib = array.array("q", [v for r in rows for v in r]), array.array("d", COEF), L.lib()
+    at = table.buffer_info()[0]
+    size = lib.dvae_newton_schulz_workspace_bytes(at, len(rows))
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    L.check(lib.dvae_muon_step(at, len(rows), lr, mu, 1, 0.0, L.MUON_SPECTRAL, coef.buffer_info()[0], 5, 1e-7, ws.data_ptr(), size,
+                               L.stream()))
+    # a handful of roundings of fp32 each: 2^-24 of the largest term, |p| or |m|
+    assert float((m[0].double() - m64).abs().max()) <= 4 * 2.0 ** -24 * float(m64.abs().max() + g[0].abs().max())
+    assert float((p[0].double() - p64).abs().max()) <= 4 * 2.0 ** -24 * float(p64.abs().max() + p[0].abs().max())
+
+
 def test_vectors_only_and_views_of_a_bucket():
     step_held([(7,), (), (5000,)])
     shapes = [(3,), (33, 17), (64, 2, 3), (1,), (40, 41)]

@@ -35,6 +35,13 @@ def test_layer_norm_refuses_bad_arguments():
     assert lib.dvae_layer_norm_workspace_bytes(-1, 8, L.F32) == 0 and lib.dvae_layer_norm_workspace_bytes(4, 0, L.F32) == 0
 
 
+def test_layer_norm_refuses_rows_of_which_two_leave_32_bits():
+    lib, c = L.lib(), 1 << 30
+    assert lib.dvae_layer_norm_fwd(F, c, None, None, F, c, None, None, 1, c, 1e-5, L.F32, None) == -1
+    assert lib.dvae_layer_norm_bwd(F, c, F, c, None, F, F, F, c, F, None, F, 1 << 40, 1, c, L.F32, None) == -1
+    assert lib.dvae_layer_norm_workspace_bytes(1, c, L.F32) == 0 and lib.dvae_layer_norm_workspace_bytes(1, c - 1, L.F32) >= 8 * (c - 1)
+
+
 def test_newton_schulz_and_muon_refuse_bad_arguments():
     lib = L.lib()
     good = (F, F, F, 6, 8, 8, 8, 0)
