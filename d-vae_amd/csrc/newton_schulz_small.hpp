@@ -15,6 +15,7 @@
 namespace dvae {
 
 using f16x4 = __attribute__((ext_vector_type(4))) _Float16;
+using f32x2 = __attribute__((ext_vector_type(2))) float;
 
 constexpr int NS_SMALL_P = 64, NS_SMALL_Q = 768, NS_SMALL_VEC = 1 << 15, NS_SMALL_JOBS = 32;
 
@@ -29,17 +30,26 @@ struct NsSmallArgs {
 static_assert(sizeof(NsSmallArgs) <= 4096, "kernel arguments");
 
 struct NsSmallLds {
-    // A wave's partial Gram subtiles, four rows of a lane's column at a time: [3][4][lane][4].  Between two Grams the wave's
-    // transposition patch lies in them: [32 q] rows of 64 h's and 64 l's of p, PITCH bytes apart (16-byte reads of 16 rows meet
-    // all banks once), or of 64 floats while the matrix comes and goes.
+    // A wave's partial Gram subtiles, two rows of a lane's column at a time: [3][8][lane][2].  Between two Grams the wave's
+    // transposition patch lies in them: [32 q] rows of 64 (h, l) pairs of p, sixteen 16-byte chunks stored at chunk ^ turn(row)
+    // (writes of 32 pairs in two rows 4 apart and reads of a chunk of sixteen rows meet all banks once), or, PITCH bytes apart, of
+    // 64 floats while the matrix comes and goes.
     static constexpr int PITCH = 272;
-    f32x4 sum[8][3 * 4 * 64];
+    f32x2 sum[8][3 * 8 * 64];
     char a[64 * 256], b[64 * 256];                        // plane pairs, [line][row], chunks swizzled as in NsTile
     double red[8];
 };
 
 // 16-byte chunk `chunk` of row `row` of line `line`
 __device__ inline int ns_small_at(int line, int row, int chunk) { return (line * 64 + row) * 128 + ((chunk ^ (row >> 1 & 7)) << 4); }
+
+// The lane, for a phase of a step.  Addresses are worked out anew in every one: the compiler would hold some hundred of them over
+// the loop, in registers that the matrix needs.
+__device__ inline int ns_lane() {
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
 
 struct NsBlock {
     f16x8 h[2][2], l[2][2];                               // [32 rows of p][half of the block's q]
@@ -55,7 +65,7 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
     const auto x = as_global<const T>(j.x);
     const auto out = as_global<T>(j.out);
     const auto mom = as_global<float>(j.mom);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
     if (MUON && j.vec) {
         for (long e = threadIdx.x; e < (long)m * n; e += 512) {
             const float gr = (float)x[e], p = (float)out[e];
@@ -163,13 +173,9 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
 
     const int used = min(8, (q + 31) / 32);               // waves that own a block
     for (int step = 0; step < g.steps; ++step) {
-        // Addresses are worked out anew in every step: the compiler would hold some hundred of them over the loop, in registers
-        // that the matrix needs.
-        int lane = threadIdx.x & 63;
-        asm volatile("" : "+v"(lane));
-        const int col = lane & 31, half = lane >> 5;
         // ---- Gram ----
         if (wave < used) {
+            const int lane = ns_lane();
             f32x16 acc[3];
 #pragma unroll
             for (int t = 0; t < 3; ++t)
@@ -195,44 +201,55 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
 #pragma unroll
             for (int t = 0; t < 3; ++t)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    s.sum[wave][(t * 4 + e) * 64 + lane] = f32x4{acc[t][4 * e], acc[t][4 * e + 1], acc[t][4 * e + 2], acc[t][4 * e + 3]};
+                for (int e = 0; e < 8; ++e) s.sum[wave][(t * 8 + e) * 64 + lane] = f32x2{acc[t][2 * e], acc[t][2 * e + 1]};
         }
         __syncthreads();
-        // ---- A: twelve groups of four rows of a subtile, to waves 0 .. 7 and 0 .. 3 ----
-        for (int task = wave; task < 12; task += 8) {
-            f32x4 part[8];
+        // ---- A: two rows of each subtile a lane ----
+        {
+            const int lane = ns_lane(), col = lane & 31, half = lane >> 5, part = wave & 1;
+            f32x2 v[3];
+            if (used == 8) {
 #pragma unroll
-            for (int w = 0; w < 8; ++w) {
-                part[w] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if (w < used) part[w] = s.sum[w][task * 64 + lane];
+                for (int t = 0; t < 3; ++t) {
+                    f32x2 f[8];
+#pragma unroll
+                    for (int w = 0; w < 8; ++w) f[w] = s.sum[w][(t * 8 + wave) * 64 + lane];
+                    v[t] = ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+                }
+            } else {
+#pragma unroll
+                for (int t = 0; t < 3; ++t) v[t] = s.sum[0][(t * 8 + wave) * 64 + lane];
+                for (int w = 1; w < used; ++w)
+#pragma unroll
+                    for (int t = 0; t < 3; ++t) v[t] += s.sum[w][(t * 8 + wave) * 64 + lane];
             }
-            const f32x4 v = ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
-            const int t = task >> 2;
-            const int row = (t ? 32 : 0) + 8 * (task & 3) + 4 * half, c = (t == 2 ? 32 : 0) + col;
-            f16x4 h, l;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float f = ns_rounded(v[i] * (NS_SA / (NS_SX * NS_SX)));
-                h[i] = (f16)f;
-                l[i] = (f16)(f - (float)h[i]);
-            }
-            // the lane's four rows of column c are four columns of row c; the subtile below the diagonal is stored as it is, too
-            const int chunk = (row & 31) >> 3;
-            *reinterpret_cast<f16x4*>(s.a + ns_small_at(row >> 5, c, chunk) + (row & 7) * 2) = h;
-            *reinterpret_cast<f16x4*>(s.a + ns_small_at(row >> 5, c, 4 + chunk) + (row & 7) * 2) = l;
-            if (t == 1) {
+            for (int t = 0; t < 3; ++t) {
+                const int row = (t ? 32 : 0) + 8 * (wave >> 1) + 4 * half + 2 * part, c = (t == 2 ? 32 : 0) + col;
+                f16x2 h, l;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    *reinterpret_cast<f16*>(s.a + ns_small_at(0, row + i, c >> 3) + (c & 7) * 2) = h[i];
-                    *reinterpret_cast<f16*>(s.a + ns_small_at(0, row + i, 4 + (c >> 3)) + (c & 7) * 2) = l[i];
+                for (int i = 0; i < 2; ++i) {
+                    const float f = ns_rounded(v[t][i] * (NS_SA / (NS_SX * NS_SX)));
+                    h[i] = (f16)f;
+                    l[i] = (f16)(f - (float)h[i]);
+                }
+                // the lane's two rows of column c are two columns of row c; the subtile below the diagonal is stored as it is, too
+                const int chunk = wave >> 1;
+                *reinterpret_cast<f16x2*>(s.a + ns_small_at(row >> 5, c, chunk) + (row & 7) * 2) = h;
+                *reinterpret_cast<f16x2*>(s.a + ns_small_at(row >> 5, c, 4 + chunk) + (row & 7) * 2) = l;
+                if (t == 1) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        *reinterpret_cast<f16*>(s.a + ns_small_at(0, row + i, c >> 3) + (c & 7) * 2) = h[i];
+                        *reinterpret_cast<f16*>(s.a + ns_small_at(0, row + i, 4 + (c >> 3)) + (c & 7) * 2) = l[i];
+                    }
                 }
             }
         }
         __syncthreads();
         // ---- square: two 16x16 subtiles a wave, their lines a 16x16x32 MFMA each ----
         {
-            const int r16 = lane & 15, quarter = lane >> 4;
+            const int lane = ns_lane(), r16 = lane & 15, quarter = lane >> 4;
             const float s2 = g.c * (NS_SB / (NS_SA * NS_SA)), s1 = g.b * (NS_SB / NS_SA), s0 = g.a * NS_SB;
             const int ti = wave >> 1;
             f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -275,7 +292,9 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
         }
         __syncthreads();
         // ---- apply ----
+        const int lane = ns_lane(), col = lane & 31, half = lane >> 5;
         char* xt = reinterpret_cast<char*>(s.sum[wave]);
+        const int turn = (col & 3) | (col >> 3 & 1) << 2 | (col >> 2 & 1) << 3;
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
             const int q0 = (wave + 8 * k) * 32;
@@ -283,10 +302,11 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        char* at = xt + (8 * (e >> 2) + 4 * half + (e & 3)) * NsSmallLds::PITCH + (i * 32 + col) * 2;
-                        *reinterpret_cast<f16*>(at) = blk[k].h[i][e >> 3][e & 7];
-                        *reinterpret_cast<f16*>(at + 128) = blk[k].l[i][e >> 3][e & 7];
+                    for (int e = 0; e < 8; ++e) {         // rows 8 (e / 4) + 4 half + e % 4 and 16 further down
+                        char* at = xt + (8 * (e >> 2) + 4 * half + (e & 3)) * 256 + (((i * 8 + (col >> 2)) ^ (half << 3) ^ e) << 4) + (col & 3) * 4;
+#pragma unroll
+                        for (int t = 0; t < 2; ++t)
+                            *reinterpret_cast<f16x2*>(at + t * 16 * 256) = f16x2{blk[k].h[i][t][e], blk[k].l[i][t][e]};
                     }
                 ns_wave_sync();
                 f32x16 acc[2];
@@ -297,8 +317,13 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk) {
                     const int line = kk >> 1, t = kk & 1;
-                    const f16x8 lh = *reinterpret_cast<const f16x8*>(xt + col * NsSmallLds::PITCH + kk * 32 + half * 16);
-                    const f16x8 ll = *reinterpret_cast<const f16x8*>(xt + col * NsSmallLds::PITCH + 128 + kk * 32 + half * 16);
+                    f16x8 lh, ll;
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const f16x8 v = *reinterpret_cast<const f16x8*>(xt + col * 256 + (((kk * 4 + half * 2 + c) ^ turn) << 4));
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) { lh[c * 4 + i] = v[2 * i]; ll[c * 4 + i] = v[2 * i + 1]; }
+                    }
                     f16x8 rh[2], rl[2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
