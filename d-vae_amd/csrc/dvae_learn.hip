@@ -215,6 +215,7 @@ bool ns_all_small(const dvae_matrix* mats, int count) {
     for (int i = 0; i < count; ++i) {
         const int64_t p = mats[i].rows < mats[i].cols ? mats[i].rows : mats[i].cols, q = mats[i].rows < mats[i].cols ? mats[i].cols : mats[i].rows;
         if (mats[i].vector ? mats[i].rows * mats[i].cols > NS_SMALL_VEC : p > NS_SMALL_P || q > NS_SMALL_Q) return false;
+        if (mats[i].x_stride > NS_SMALL_SPAN / mats[i].rows || mats[i].out_stride > NS_SMALL_SPAN / mats[i].rows) return false;
     }
     return true;
 }

@@ -18,6 +18,7 @@ using f16x4 = __attribute__((ext_vector_type(4))) _Float16;
 using f32x2 = __attribute__((ext_vector_type(2))) float;
 
 constexpr int NS_SMALL_P = 64, NS_SMALL_Q = 768, NS_SMALL_VEC = 1 << 15, NS_SMALL_JOBS = 32;
+constexpr long NS_SMALL_SPAN = 1L << 28;                  // elements between a matrix's first and last: offsets of 32 bits
 
 struct NsSmallArgs {
     NsJob jobs[NS_SMALL_JOBS];
@@ -61,17 +62,16 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
     NsSmallLds& s = *reinterpret_cast<NsSmallLds*>(smem);
     const NsJob j = g.table ? g.table[blockIdx.x] : g.jobs[blockIdx.x];
     const int m = j.m, n = j.n;
-    const long xs = j.xs, os = j.os;
-    const auto x = as_global<const T>(j.x);
-    const auto out = as_global<T>(j.out);
-    const auto mom = as_global<float>(j.mom);
+    const cgbytes x = as_global<const char>(j.x);
+    const gbytes out = as_global<char>(j.out), mom = as_global<char>(j.mom);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
     if (MUON && j.vec) {
-        for (long e = threadIdx.x; e < (long)m * n; e += 512) {
-            const float gr = (float)x[e], p = (float)out[e];
-            const float mi = g.mu * mom[e] + g.nu * gr;
-            mom[e] = mi;
-            out[e] = (T)(p * g.decay - g.lr * (g.nesterov ? g.nu * gr + g.mu * mi : mi));
+        const auto gr = as_global<const float>(j.x);
+        const auto par = as_global<float>(j.out), mo = as_global<float>(j.mom);
+        for (int e = threadIdx.x; e < m * n; e += 512) {
+            const float mi = g.mu * mo[e] + g.nu * gr[e];
+            mo[e] = mi;
+            par[e] = par[e] * g.decay - g.lr * (g.nesterov ? g.nu * gr[e] + g.mu * mi : mi);
         }
         return;
     }
@@ -81,12 +81,23 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
     float* patch = reinterpret_cast<float*>(s.sum[wave]);
 
     // A block's elements as the caller's memory has them along lanes: a tall matrix's rows hold p (one q at a time), another's
-    // q (32 of two p's).  Element i of half t is (qi, pi) of the block, at start + i * leap.
-    auto qi_of = [&](int t, int i) { return tall ? t * 16 + i : col; };
-    auto pi_of = [&](int t, int i) { return tall ? lane : (t * 16 + i) * 2 + half; };
-    auto start_of = [&](int q0, int t, long stride) {
-        return tall ? (long)(q0 + t * 16) * stride + lane : (long)(t * 32 + half) * stride + q0 + col;
+    // q (32 of two p's).  Of the sixteen of half t a lane has the first `count`, `leap` apart from `at` on (bytes; the host sees
+    // to it that they fit 32 bits); those that do not exist read the first one of all and count as zero.
+    struct Half {
+        int count;
+        unsigned at;
     };
+    auto half_of = [&](int q0, int t, unsigned stride) {
+        Half r;
+        r.count = tall ? (lane < p ? q - q0 - t * 16 : 0) : (q0 + col < q ? (p - t * 32 - half + 1) >> 1 : 0);
+        const unsigned at = (tall ? (q0 + t * 16) * stride + lane : (t * 32 + half) * stride + q0 + col) * (unsigned)sizeof(T);
+        r.at = r.count > 0 ? at : 0u;
+        return r;
+    };
+    const unsigned xleap = (unsigned)(tall ? j.xs : 2 * j.xs) * (unsigned)sizeof(T), oleap = (unsigned)(tall ? j.os : 2 * j.os) * (unsigned)sizeof(T);
+    // where they lie in the patch, [q][p]
+    const int patch_leap = tall ? PITCH : 2;
+    auto patch_of = [&](int t) { return patch + (tall ? t * 16 * PITCH + lane : col * PITCH + t * 32 + half); };
 
     // ---- load, all of it in flight at once; then u and its norm, and through the patch to [q][p] ---------------------
     float raw[NB][2][16];
@@ -96,10 +107,9 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
         const int q0 = (wave + 8 * k) * 32;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const long start = start_of(q0, t, xs), leap = tall ? xs : 2 * xs;
+            const Half f = half_of(q0, t, (unsigned)j.xs);
 #pragma unroll
-            for (int i = 0; i < 16; ++i)                  // elements past the edge read the first one and count as zero
-                raw[k][t][i] = (float)x[q0 + qi_of(t, i) < q && pi_of(t, i) < p ? start + i * leap : 0L];
+            for (int i = 0; i < 16; ++i) raw[k][t][i] = (float)*(const DVAE_GLOBAL T*)(x + (f.at + (i < f.count ? i * xleap : 0u)));
         }
     }
 #pragma unroll
@@ -108,23 +118,24 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
         if (q0 < q) {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const long start = start_of(q0, t, xs), leap = tall ? xs : 2 * xs;
+                const Half f = half_of(q0, t, (unsigned)j.xs);
+                float* to = patch_of(t);
                 float mv[16];
                 if (MUON) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) mv[i] = mom[q0 + qi_of(t, i) < q && pi_of(t, i) < p ? start + i * leap : 0L];
+                    for (int i = 0; i < 16; ++i) mv[i] = *(const DVAE_GLOBAL float*)(mom + (f.at + (i < f.count ? i * xleap : 0u)));
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const bool in = q0 + qi_of(t, i) < q && pi_of(t, i) < p;
+                    const bool in = i < f.count;
                     float v = in ? raw[k][t][i] : 0.f;
                     if (MUON) {
                         const float mi = in ? g.mu * mv[i] + g.nu * v : 0.f;
-                        if (in) mom[start + i * leap] = mi;
+                        if (in) *(DVAE_GLOBAL float*)(mom + (f.at + i * xleap)) = mi;
                         v = g.nesterov ? g.nu * v + g.mu * mi : mi;
                     }
                     sq += (double)v * (double)v;
-                    patch[qi_of(t, i) * PITCH + pi_of(t, i)] = v;
+                    to[i * patch_leap] = v;
                 }
             }
             ns_wave_sync();
@@ -364,16 +375,17 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
             ns_wave_sync();
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const long start = start_of(q0, t, os), leap = tall ? os : 2 * os;
+                const Half f = half_of(q0, t, (unsigned)j.os);
+                const float* from = patch_of(t);
                 float old[16];
                 if (MUON) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) old[i] = (float)out[q0 + qi_of(t, i) < q && pi_of(t, i) < p ? start + i * leap : 0L];
+                    for (int i = 0; i < 16; ++i) old[i] = (float)*(const DVAE_GLOBAL T*)(out + (f.at + (i < f.count ? i * oleap : 0u)));
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float v = patch[qi_of(t, i) * PITCH + pi_of(t, i)];
-                    if (q0 + qi_of(t, i) < q && pi_of(t, i) < p) out[start + i * leap] = (T)(MUON ? old[i] * g.decay - step_len * v : v);
+                    const float v = from[i * patch_leap];
+                    if (i < f.count) *(DVAE_GLOBAL T*)(out + (f.at + i * oleap)) = (T)(MUON ? old[i] * g.decay - step_len * v : v);
                 }
             }
             ns_wave_sync();
