@@ -165,31 +165,38 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs g) {
     const auto mom = as_global<float>(j.mom), par = as_global<float>(j.out);
     double s = 0.0;
     for (long base = (long)chunk * NS_CHUNK; base < n; base += (long)j.nchunk * NS_CHUNK) {
-        float v[16];
+        // Loads are of elements that exist, whatever becomes of their values, and whole trips store without a condition: a condition
+        // is a branch, and sixteen branches are sixteen latencies.
+        const bool whole = base + NS_CHUNK <= n;
+        float v[16], m[16], p[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const long e = base + i * 256 + threadIdx.x;
-            long at = e;
-            if (!MUON && j.xs != j.n) at = (unsigned)e / (unsigned)j.n * j.xs + (unsigned)e % (unsigned)j.n;
-            v[i] = e < n ? (float)x[at] : 0.f;
+            const long e = base + i * 256 + threadIdx.x, to = e < n ? e : 0;
+            long at = to;
+            if (!MUON && j.xs != j.n) at = (unsigned)to / (unsigned)j.n * j.xs + (unsigned)to % (unsigned)j.n;
+            v[i] = (float)x[at];
+            if (MUON) m[i] = mom[to];
+            if (MUON && j.vec) p[i] = par[to];
         }
         if (MUON) {
-            float m[16], p[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const long e = base + i * 256 + threadIdx.x;
-                m[i] = e < n ? mom[e] : 0.f;
-                p[i] = e < n && j.vec ? par[e] : 0.f;
+                m[i] = ns_rounded(ns_momentum(g, v[i], m[i]));
+                v[i] = ns_update(g, v[i], m[i]);
+                if (j.vec) p[i] = ns_rounded(p[i] * g.decay - g.lr * v[i]);
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const long e = base + i * 256 + threadIdx.x;
-                const float mi = ns_momentum(g, v[i], m[i]);
-                if (e < n) mom[e] = mi;
-                v[i] = ns_update(g, v[i], mi);
-                if (e < n && j.vec) par[e] = p[i] * g.decay - g.lr * v[i];
+                if (whole || e < n) {
+                    mom[e] = m[i];
+                    if (j.vec) par[e] = p[i];
+                }
             }
         }
+        if (!whole)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = base + i * 256 + threadIdx.x < n ? v[i] : 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) s += (double)v[i] * (double)v[i];
     }
@@ -220,17 +227,19 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsArgs g) {
     const int ncol = ns_pad(j.n) >> 6;
     const int r0 = t / ncol * 64, c0 = t % ncol * 64;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int c = c0 + lane;
+    float v[16], mom[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {                        // past the edges the last elements, which count as zero
+        const long e = (long)min(r0 + i * 4 + wave, j.m - 1) * j.xs + min(c, j.n - 1);
+        v[i] = (float)as_global<const T>(j.x)[e];
+        if (MUON) mom[i] = as_global<float>(j.mom)[e];
+    }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        const int r = r0 + i * 4 + wave, c = c0 + lane;
-        float v = 0.f;
-        if (r < j.m && c < j.n) {
-            const long e = (long)r * j.xs + c;
-            v = (float)as_global<const T>(j.x)[e];
-            if (MUON) v = ns_update(g, v, as_global<float>(j.mom)[e]);
-            v = (float)((double)v * inv);
-        }
-        tile[i * 4 + wave][lane] = ns_split(v);
+        if (MUON) v[i] = ns_update(g, v[i], mom[i]);
+        v[i] = (float)((double)v[i] * inv);
+        tile[i * 4 + wave][lane] = ns_split(r0 + i * 4 + wave < j.m && c < j.n ? v[i] : 0.f);
     }
     __syncthreads();
     // a wave writes 16 columns of 64 rows: first in the source's orientation, then in the other
@@ -788,16 +797,23 @@ __global__ __launch_bounds__(256 * G, G == 1 ? 2 : 1) void ns_last_kernel(NsArgs
             float p[16];
             if (MUON) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int row = ti * TS + NsTile<TS>::row_of(i, e);
-                    p[e] = row < j.m ? (float)out[row * j.os + col] : 0.f;
-                }
+                for (int e = 0; e < 16; ++e) p[e] = (float)out[min(ti * TS + NsTile<TS>::row_of(i, e), j.m - 1) * j.os + col];
             }
+            const bool whole = ti * TS + NsTile<TS>::row_of(i, 15) < j.m;      // a lane's last row
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const int row = ti * TS + NsTile<TS>::row_of(i, e);
                 const float v = c.acc[i][k][e] * (1.f / (NS_SB * NS_SX));
-                if (row < j.m) out[row * j.os + col] = (T)(MUON ? p[e] * g.decay - step * v : v);
+                p[e] = ns_rounded(MUON ? p[e] * g.decay - step * v : v);
+            }
+            if (whole) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) out[(ti * TS + NsTile<TS>::row_of(i, e)) * j.os + col] = (T)p[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int row = ti * TS + NsTile<TS>::row_of(i, e);
+                    if (row < j.m) out[row * j.os + col] = (T)p[e];
+                }
             }
         }
 }

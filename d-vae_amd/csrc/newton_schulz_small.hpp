@@ -94,6 +94,17 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
         r.at = r.count > 0 ? at : 0u;
         return r;
     };
+    // Stores of the elements that exist: of all sixteen in one run where a lane has them, else a branch each.
+    auto put = [&](const Half& f, auto&& store) {
+        if (f.count >= 16) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) store(i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (i < f.count) store(i);
+        }
+    };
     const unsigned xleap = (unsigned)(tall ? j.xs : 2 * j.xs) * (unsigned)sizeof(T), oleap = (unsigned)(tall ? j.os : 2 * j.os) * (unsigned)sizeof(T);
     // where they lie in the patch, [q][p]
     const int patch_leap = tall ? PITCH : 2;
@@ -130,13 +141,13 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
                     const bool in = i < f.count;
                     float v = in ? raw[k][t][i] : 0.f;
                     if (MUON) {
-                        const float mi = in ? g.mu * mv[i] + g.nu * v : 0.f;
-                        if (in) *(DVAE_GLOBAL float*)(mom + (f.at + i * xleap)) = mi;
-                        v = g.nesterov ? g.nu * v + g.mu * mi : mi;
+                        mv[i] = ns_rounded(in ? g.mu * mv[i] + g.nu * v : 0.f);
+                        v = g.nesterov ? g.nu * v + g.mu * mv[i] : mv[i];
                     }
                     sq += (double)v * (double)v;
                     to[i * patch_leap] = v;
                 }
+                if (MUON) put(f, [&](int i) { *(DVAE_GLOBAL float*)(mom + (f.at + i * xleap)) = mv[i]; });
             }
             ns_wave_sync();
         }
@@ -382,11 +393,12 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) old[i] = (float)*(const DVAE_GLOBAL T*)(out + (f.at + (i < f.count ? i * oleap : 0u)));
                 }
+                float v[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float v = from[i * patch_leap];
-                    if (i < f.count) *(DVAE_GLOBAL T*)(out + (f.at + i * oleap)) = (T)(MUON ? old[i] * g.decay - step_len * v : v);
-                }
+                for (int i = 0; i < 16; ++i) v[i] = from[i * patch_leap];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[i] = ns_rounded(MUON ? old[i] * g.decay - step_len * v[i] : v[i]);
+                put(f, [&](int i) { *(DVAE_GLOBAL T*)(out + (f.at + i * oleap)) = (T)v[i]; });
             }
             ns_wave_sync();
         }
