@@ -312,6 +312,8 @@ struct NsTile {
         }
     }
     // `lines` is even; rows past lrows / rrows re-read the last one: their results are not stored
+    // SAME: both operands are the same rows, staged once.
+    template <bool SAME = false>
     __device__ inline void run(cgbytes L, int lrows, int l0, cgbytes R, int rrows, int r0, int line0, int lines, char* smem) {
         const int tid = threadIdx.x & 255, row = tid & 31, chunk = tid >> 5, group = threadIdx.x >> 8;
         const int lane = tid & 63, wave = tid >> 6;
@@ -338,7 +340,7 @@ struct NsTile {
 #pragma unroll
             for (int i = 0; i < PASS; ++i) {
                 s.l[i] = *(const DVAE_GLOBAL u32x4*)lp[i];
-                s.r[i] = *(const DVAE_GLOBAL u32x4*)rp[i];
+                if (!SAME) s.r[i] = *(const DVAE_GLOBAL u32x4*)rp[i];
             }
             const bool more = --ahead > 0;
 #pragma unroll
@@ -353,12 +355,12 @@ struct NsTile {
 #pragma unroll
             for (int i = 0; i < PASS; ++i) {
                 *reinterpret_cast<u32x4*>(s + i * 32 * 128) = l.l[i];
-                *reinterpret_cast<u32x4*>(s + TS * 128 + i * 32 * 128) = l.r[i];
+                if (!SAME) *reinterpret_cast<u32x4*>(s + TS * 128 + i * 32 * 128) = l.r[i];
             }
         };
         const int half = lane >> 5, sw = lane >> 1 & 7;
         const char* sL = smem + ((wave >> 1) * (TS / 2) + (lane & 31)) * 128;
-        const char* sR = smem + TS * 128 + ((wave & 1) * (TS / 2) + (lane & 31)) * 128;
+        const char* sR = smem + (SAME ? 0 : TS * 128) + ((wave & 1) * (TS / 2) + (lane & 31)) * 128;
         auto read = [&](Frags& f, int at, int k) {
             const int ch = at * (2 * TS * 128) + (((k * 2 + half) ^ sw) << 4), cl = at * (2 * TS * 128) + (((4 + k * 2 + half) ^ sw) << 4);
 #pragma unroll
@@ -480,6 +482,17 @@ __device__ inline void ns_triangle(int t, int& i, int& k) {
     k = t - i * (i + 1) / 2;
 }
 
+// tile t of `side` rows of tiles: those below the diagonal row by row, then the diagonal
+__device__ inline void ns_diagonal_last(int t, int side, int& i, int& k) {
+    const int below = side * (side - 1) / 2;
+    if (t >= below) {
+        i = k = t - below;
+    } else {
+        ns_triangle(t, i, k);
+        ++i;
+    }
+}
+
 // The symmetric products store the tiles at and below the diagonal and their mirror images.  Tiles on the diagonal are
 // stored once: their two halves agree to rounding only, and two writers of one place would leave either's.
 template <int TS>
@@ -524,6 +537,13 @@ __device__ inline void ns_symmetric_value(const NsArgs& g, const NsPlanes& w, f3
     }
 }
 
+// One matrix in whole tiles: those on the diagonal, cheaper by half their loads, are spread over the XCDs by themselves and come last,
+// so that they are what a CU with a tile more than the others has more (2048 x 2048, 528 tiles on 256 CUs: 775 -> 755 us; in line
+// with the others, all on the last XCD, 780).
+__device__ inline int ns_spread(const NsArgs& g, int ts, bool pieces) {
+    return pieces || g.njobs != 1 ? g.total : g.total - (ns_pad(min(g.one.m, g.one.n)) + ts - 1) / ts;
+}
+
 // The symmetric products, tiles at and below the diagonal: whole or (Gram, where the tiles alone would leave much of the chip
 // idle) in pieces of the contraction, a job's kc lines each, that leave fp32 partial tiles for ns_gram_sum_kernel.  Neighbouring
 // workgroups take different tiles of the same lines: an XCD reads a part of X once.
@@ -532,16 +552,18 @@ __global__ __launch_bounds__(256, 2) void ns_symmetric_kernel(NsArgs g) {
     extern __shared__ __align__(16) char smem[];
     constexpr int S = NsTile<TS>::S;
     int t, ti, tk;
-    const int wg = ns_swizzle(blockIdx.x, g.total);
+    const int spread = ns_spread(g, TS, PIECES), wg = (int)blockIdx.x < spread ? ns_swizzle(blockIdx.x, spread) : blockIdx.x;
     const NsJob j = ns_job_of(g, ns_find(g, SQUARE ? NS_SQUARE : NS_GRAM, wg, t));
     const NsPlanes w(g, j);
     const int side = (w.P + TS - 1) / TS, tiles = side * (side + 1) / 2;
     const int lines = (SQUARE ? w.P : w.Q) / 32, kc = j.kc, line0 = PIECES ? t / tiles * kc : 0;
-    ns_triangle(PIECES ? t % tiles : t, ti, tk);
+    ns_diagonal_last(PIECES ? t % tiles : t, side, ti, tk);
     NsTile<TS> c;
     c.zero();
     const cgbytes m = SQUARE ? w.a : w.x;
-    c.run(m, w.P, ti * TS, m, w.P, tk * TS, line0, PIECES ? min(kc, lines - line0) : lines, smem);
+    const int n = PIECES ? min(kc, lines - line0) : lines;
+    if (ti == tk) c.template run<true>(m, w.P, ti * TS, m, w.P, tk * TS, line0, n, smem);
+    else c.run(m, w.P, ti * TS, m, w.P, tk * TS, line0, n, smem);
     if (PIECES) {
         const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
         const auto out = as_global<float>(g.part) + (long)wg * (TS * TS) + lane * 4;
@@ -579,10 +601,10 @@ __global__ __launch_bounds__(256) void ns_gram_sum_kernel(NsArgs g) {
     const int jn = ns_find(g, NS_GRAM_TILES, blockIdx.x / SUBS, t);
     const NsJob j = ns_job_of(g, jn);
     const NsPlanes w(g, j);
-    ns_triangle(t, ti, tk);
+    const int side = (w.P + TS - 1) / TS, tiles = side * (side + 1) / 2;
+    ns_diagonal_last(t, side, ti, tk);
     const int row = ti * TS + sub / (TS / 32) * 32, col = tk * TS + sub % (TS / 32) * 32;
     if (row >= w.P || col >= w.P) return;
-    const int side = (w.P + TS - 1) / TS, tiles = side * (side + 1) / 2;
     const int pieces = (w.Q / 32 + j.kc - 1) / j.kc;
     const auto in = as_global<const float>(g.part) + ((g.njobs == 1 ? 0L : (long)g.first[NS_GRAM * g.jp + jn]) + t) * (TS * TS) + sub * 1024 + lane * 4;
     f32x4 v[4] = {};
