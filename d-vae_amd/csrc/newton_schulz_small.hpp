@@ -1,6 +1,7 @@
 // The whole iteration of a small matrix (p <= 64, q <= 768) in one workgroup and one launch: momentum, norm, every step, the
 // result or the parameter's update.  What bounds such matrices is not work (64 x 576: 0.3 GFLOP of MFMAs) but the chain of
-// dependent launches, four a step through the batched kernels, about 5 us each.
+// dependent launches, four a step through the batched kernels, about 5 us each.  Measured: 64 x 576 45.5 us (6.7 a step), 64 x 27 19.5
+// (2.9 a step); what a step waits for is the chain of latencies below, and, with several blocks a wave, their conversions.
 //
 // Eight waves; wave w owns the 32-column blocks w, w + 8, .. of X (NB at most) and keeps them in registers for good, as
 // MFMA fragments: a product's accumulator X^T[q][p] has p across lanes and q down the registers, which is an operand of
