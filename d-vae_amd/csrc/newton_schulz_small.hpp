@@ -1,7 +1,7 @@
 // The whole iteration of a small matrix (p <= 64, q <= 768) in one workgroup and one launch: momentum, norm, every step, the
 // result or the parameter's update.  What bounds such matrices is not work (64 x 576: 0.3 GFLOP of MFMAs) but the chain of
-// dependent launches, four a step through the batched kernels, about 5 us each.  Measured: 64 x 576 45.5 us (6.7 a step), 64 x 27 19.5
-// (2.9 a step); what a step waits for is the chain of latencies below, and, with several blocks a wave, their conversions.
+// dependent launches, four a step through the batched kernels, about 5 us each.  Measured: 64 x 576 47 us (7 a step), 64 x 27 20.5
+// (3 a step); what a step waits for is the chain of latencies below, and, with several blocks a wave, their conversions.
 //
 // Eight waves; wave w owns the 32-column blocks w, w + 8, .. of X (NB at most) and keeps them in registers for good, as
 // MFMA fragments: a product's accumulator X^T[q][p] has p across lanes and q down the registers, which is an operand of
@@ -39,6 +39,7 @@ struct NsSmallLds {
     static constexpr int PITCH = 272;
     f32x2 sum[8][3 * 8 * 64];
     char a[64 * 256], b[64 * 256];                        // plane pairs, [line][row], chunks swizzled as in NsTile
+    float diag[64];                                       // of A, see ns_polynomial
     double red[8];
 };
 
@@ -252,7 +253,11 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
                 f16x2 h, l;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const float f = ns_rounded(v[t][i] * (NS_SA / (NS_SX * NS_SX)));
+                    float f = ns_rounded(v[t][i] * (NS_SA / (NS_SX * NS_SX)));
+                    if (t != 1 && row + i == c) {
+                        s.diag[c] = f;
+                        f = 0.f;
+                    }
                     h[i] = (f16)f;
                     l[i] = (f16)(f - (float)h[i]);
                 }
@@ -273,7 +278,6 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
         // ---- square: two 16x16 subtiles a wave, their lines a 16x16x32 MFMA each ----
         {
             const int lane = ns_lane(), r16 = lane & 15, quarter = lane >> 4;
-            const float s2 = g.c * (NS_SB / (NS_SA * NS_SA)), s1 = g.b * (NS_SB / NS_SA), s0 = g.a * NS_SB;
             const int ti = wave >> 1;
             f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
@@ -300,12 +304,12 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
                 const int c = ((wave & 1) * 2 + n) * 16 + r16, r0 = ti * 16 + 4 * quarter;
                 const int ah = ns_small_at(r0 >> 5, c, (r0 & 31) >> 3) + (r0 & 7) * 2, al = ns_small_at(r0 >> 5, c, 4 + ((r0 & 31) >> 3)) + (r0 & 7) * 2;
                 const f16x4 vh = *reinterpret_cast<const f16x4*>(s.a + ah), vl = *reinterpret_cast<const f16x4*>(s.a + al);
+                const float dc = s.diag[c];
+                const f32x4 dr = *reinterpret_cast<const f32x4*>(s.diag + r0);
                 f16x4 h, l;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    float r = s2 * acc[n][i] + s1 * ((float)vh[i] + (float)vl[i]);
-                    if (r0 + i == c) r += s0;
-                    r = ns_rounded(r);
+                    const float r = ns_rounded(ns_polynomial(g, acc[n][i], (float)vh[i] + (float)vl[i], dr[i], dc, r0 + i == c));
                     h[i] = (f16)r;
                     l[i] = (f16)(r - (float)h[i]);
                 }
