@@ -76,6 +76,7 @@ class VAE_Trainer:
         self.monitor_every = self.log_frequency if monitor_every is None else monitor_every
         self._monitors = {k: 0.0 for k in ("loss_cls", "loss_cls_p", "loss_cls_p2", "loss_cls_purified")}
         self._monitor_fresh, self._monitor_n = False, 0
+        self._sync = None                   # gradient averaging of the generic route, made on several ranks only
         self._reset_stats()
 
     def _reset_stats(self):
@@ -114,10 +115,31 @@ class VAE_Trainer:
         loss_rec_p = F.mse_loss((rec + perturbation).clamp(0, 1), images)
         loss_p = F.mse_loss(perturbation, torch.zeros_like(perturbation))
         kld_loss = torch.mean(-0.5 * torch.sum(1 + log_var - mu ** 2 - log_var.exp(), dim=1), dim=(0, 1, 2))
-        loss = loss_rec + loss_rec_p + weight * max(kld_loss, target)
-        if epoch > 10:
-            loss = loss + max(loss_p, 0.002)
-        loss.backward()
+        _, world = D.world_info()
+        if world == 1:
+            loss = loss_rec + loss_rec_p + weight * max(kld_loss, target)
+            if epoch > 10:
+                loss = loss + max(loss_p, 0.002)
+            loss.backward()
+        else:
+            # The loss of the global batch, as the fused route computes it: its terms are means over all ranks' samples, the gates
+            # look at those, and what a rank differentiates is its own samples' part of it.
+            b, own = images.shape[0], (loss_rec, loss_rec_p, loss_p, kld_loss)
+            sums = D.allreduce_sum_(torch.stack([t.detach() * b for t in own] + [loss_rec.new_tensor(float(b))]))
+            part, total = (b * world / sums[4], own[0] + own[1])
+            loss_rec, loss_rec_p, loss_p, kld_loss = (sums[:4] / sums[4]).unbind()
+            loss = loss_rec + loss_rec_p + weight * max(kld_loss, target)
+            if not target > kld_loss:
+                total = total + weight * own[3]
+            if epoch > 10:
+                loss = loss + max(loss_p, 0.002)
+                if not 0.002 > loss_p:
+                    total = total + own[2]
+            (part * total).backward()
+            if self._sync is None:
+                from .classifier import DataParallelSGD
+                self._sync = DataParallelSGD()
+            self._sync.sync(model)
         grad_norm = torch.nn.utils.clip_grad_norm_(model.parameters(), grad_clip)
         optimizer.step()
         # The model notices in-place updates through the tensors' version counters, but writes through ``param.data``
