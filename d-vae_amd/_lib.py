@@ -8,6 +8,7 @@ import ctypes as C
 import os
 
 import torch
+import torch.autograd.forward_ad as _fwd_ad
 
 F32, BF16 = 0, 1
 OP_FWD, OP_DGRAD = 0, 1
@@ -146,6 +147,15 @@ def on_device(device):
     if _CUR_DEVICE is not None and device.index == _CUR_DEVICE():
         return _NO_GUARD
     return torch.cuda.device(device)
+
+
+def refuse_tangents(what, *tensors):
+    """Raises where a tensor carries a forward-mode tangent: a kernel sees only its value, and the result would silently have
+    none.  Outside a dual level this is one comparison."""
+    if getattr(_fwd_ad, "_current_level", 0) >= 0:
+        for t in tensors:
+            if t is not None and _fwd_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} has no forward-mode derivative, and an argument carries a tangent")
 
 
 def act_channels(c, dtype=F32):

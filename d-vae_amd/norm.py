@@ -15,6 +15,7 @@ _DTYPES = {torch.float32: L.F32, torch.bfloat16: L.BF16}
 
 
 def _check(x, weight, bias, eps):
+    L.refuse_tangents("layer_norm", x, weight, bias)
     if not x.is_cuda:
         raise RuntimeError("layer_norm runs on libdvae_hip: x must be a device tensor")
     if x.dtype not in _DTYPES:
@@ -100,7 +101,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     ``x``: float32 or bfloat16 on the device, any shape and strides; rows that are slices of wider ones (an activation map
     without its padding channels) are read in place, other layouts are copied once.  ``weight`` / ``bias``: float32 of the
     last dimension's size, or None.  The result is contiguous and of x's type.  Gradients flow to all three and can be taken
-    once (no second derivatives).  A step captured into a graph follows torch's rule for captured backward passes: no eager
+    once (no second derivatives, no forward mode).  A step captured into a graph follows torch's rule for captured backward passes: no eager
     graph of the same leaves may be alive during the capture."""
     _check(x, weight, bias, eps)
     with L.on_device(x.device):

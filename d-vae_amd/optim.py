@@ -36,6 +36,7 @@ def newton_schulz(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     accuracy for either type.  The result is not differentiable."""
     many = isinstance(x, (list, tuple))
     xs = list(x) if many else [x]
+    L.refuse_tangents("newton_schulz", *xs)
     outs, table, keep = [], array("q"), []
     for i, t in enumerate(xs):
         if not t.is_cuda:
@@ -93,6 +94,7 @@ def muon_step(params, grads, momenta, lr=0.02, momentum=0.95, nesterov=True, wei
     (gains, biases) move by lr u.  All parameters go through the same two dozen launches."""
     if not len(params) == len(grads) == len(momenta):
         raise RuntimeError(f"muon_step: {len(params)} parameters, {len(grads)} gradients, {len(momenta)} momenta")
+    L.refuse_tangents("muon_step", *params, *grads, *momenta)
     if scale not in _SCALES:
         raise RuntimeError(f"muon_step: scale {scale!r} ({sorted(_SCALES)})")
     table, written, read = array("q"), set(), set()
