@@ -79,7 +79,25 @@ def _backward(ctx, dy):
     return dx, dw, db, None
 
 
-_backward_once = torch.autograd.function.once_differentiable(_backward)
+class _FirstGradient(torch.autograd.Function):
+    """The identity on one of the gradients, as a function of the tensors it depends on: where any of them is being
+    differentiated the gradient says so (requires_grad), and its own backward raises."""
+
+    @staticmethod
+    def forward(ctx, grad, *of):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("layer_norm: its gradients can be taken once; there are no second derivatives")
+
+
+def _backward_once(ctx, dy):
+    with torch.no_grad():
+        dx, dw, db, _ = _backward(ctx, dy)
+    x, weight, _ = ctx.saved_tensors
+    return (None if dx is None else _FirstGradient.apply(dx, dy, x, weight), None if dw is None else _FirstGradient.apply(dw, dy, x),
+            None if db is None else _FirstGradient.apply(db, dy), None)
 
 
 class _LayerNormFunction(torch.autograd.Function):
