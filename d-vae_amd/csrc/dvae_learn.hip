@@ -52,6 +52,8 @@ inline int ln_bwd_groups(int64_t rows, int C, int dtype) {
     if (g > cap) g = cap;
     return (int)(g < 1 ? 1 : g);
 }
+// Workgroups of the slabs' sum, of 1024 threads: a launch holds fewer than 2^32 threads, rows may have 2^30 columns.
+constexpr int64_t LN_REDUCE_GRID = 1 << 20;
 // Forward: eight workgroups of four waves a CU, which then walk their rows with gamma / beta in registers.
 constexpr int LN_GRID = 2048;
 
@@ -531,7 +533,8 @@ int dvae_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_
         DVAE_CHECK_LAUNCH("layer_norm_bwd");
     }
     if (sums) {
-        hipLaunchKernelGGL(ln_reduce_kernel, dim3((unsigned)cdiv64(2LL * C, 64)), dim3(1024), 0, S(st), (const float*)workspace,
+        const int64_t g = std::min(cdiv64(2LL * C, 64), LN_REDUCE_GRID);
+        hipLaunchKernelGGL(ln_reduce_kernel, dim3((unsigned)g), dim3(1024), 0, S(st), (const float*)workspace,
                            rows ? groups : 0, C, dgamma, dbeta);
         DVAE_CHECK_LAUNCH("layer_norm_bwd");
     }

@@ -503,31 +503,33 @@ __global__ __launch_bounds__(256) void ln_cols_kernel(LnArgs a) {
     out[a.C + c] = db;
 }
 
-// slabs [G][2][C] -> dgamma, dbeta: 64 columns a workgroup, its 16 waves take every 16th slab, eight loads in flight each
+// slabs [G][2][C] -> dgamma, dbeta: 64 columns a workgroup at a time, its 16 waves take every 16th slab, eight loads in flight each
 __global__ __launch_bounds__(1024) void ln_reduce_kernel(const float* partial, int G, int C, float* dgamma, float* dbeta) {
     __shared__ float red[16][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int e = blockIdx.x * 64 + lane;                // index into [2][C]
-    float s = 0.f;
-    if (e < 2 * C) {
-        const float* p = partial + e;
-        const long st = 2L * C;
-        for (int g = wave; g < G; g += 128) {
-            float v[8];
+    const long st = 2L * C;
+    for (long e = (long)blockIdx.x * 64 + lane; e - lane < st; e += (long)gridDim.x * 64) {       // index into [2][C]
+        float s = 0.f;
+        if (e < st) {
+            const float* p = partial + e;
+            for (int g = wave; g < G; g += 128) {
+                float v[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = g + 16 * i < G ? p[(g + 16 * i) * st] : 0.f;
+                for (int i = 0; i < 8; ++i) v[i] = g + 16 * i < G ? p[(g + 16 * i) * st] : 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s += v[i];
+                for (int i = 0; i < 8; ++i) s += v[i];
+            }
         }
-    }
-    red[wave][lane] = s;
-    __syncthreads();
-    if (wave == 0 && e < 2 * C) {
-        s = 0.f;
+        red[wave][lane] = s;
+        __syncthreads();
+        if (wave == 0 && e < st) {
+            s = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s += red[i][lane];
-        float* out = e < C ? dgamma : dbeta;
-        if (out) out[e < C ? e : e - C] = s;
+            for (int i = 0; i < 16; ++i) s += red[i][lane];
+            float* out = e < C ? dgamma : dbeta;
+            if (out) out[e < C ? e : e - C] = s;
+        }
+        __syncthreads();
     }
 }
 
