@@ -122,7 +122,7 @@ void ln_launch(const LnArgs& a, const LnShape& s, bool bwd, int groups, hipStrea
         if (s.nv == V) ln_launch_wide<T, 16, V>(a, s, bwd, groups, st);
         else ln_launch_wide<T, 16, 2 * V>(a, s, bwd, groups, st);
     } else if (bwd) {
-        if (a.y) hipLaunchKernelGGL((ln_bwd_long_kernel<T>), dim3((int)(a.rows < 2048 ? a.rows : 2048)), dim3(1024), 0, st, a);
+        hipLaunchKernelGGL((ln_bwd_long_kernel<T>), dim3((int)(a.rows < 2048 ? a.rows : 2048)), dim3(1024), 0, st, a);
         if (a.partial) hipLaunchKernelGGL((ln_cols_kernel<T>), dim3((a.C + 255) / 256, groups), dim3(256), 0, st, a);
     } else {
         hipLaunchKernelGGL((ln_fwd_long_kernel<T>), dim3((int)(a.rows < 2048 ? a.rows : 2048)), dim3(1024), 0, st, a);
@@ -482,7 +482,8 @@ extern "C" {
 
 size_t dvae_layer_norm_workspace_bytes(int64_t rows, int C, int dtype) {
     if (rows < 0 || C <= 0 || C >= (1 << 30) || (dtype != DVAE_F32 && dtype != DVAE_BF16)) return 0;
-    return (size_t)ln_bwd_groups(rows, C, dtype) * 2 * C * sizeof(float);
+    const LnShape s = ln_shape(C, dtype);
+    return ((size_t)ln_bwd_groups(rows, C, dtype) * 2 * C + (s.lpr || s.waves ? 0 : (size_t)rows)) * sizeof(float);
 }
 
 int dvae_layer_norm_fwd(const void* x, int64_t x_stride, const float* gamma, const float* beta, void* y, int64_t y_stride,
@@ -526,6 +527,7 @@ int dvae_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_
         a.x = x; a.xs = x_stride; a.dy = dy; a.ds = dy_stride; a.y = dx; a.ys = dx_stride; a.gamma = gamma;
         a.mean = const_cast<float*>(save_mean); a.invstd = const_cast<float*>(save_invstd);
         a.partial = sums ? (float*)workspace : nullptr;
+        a.left = sums ? a.partial + (size_t)groups * 2 * C : nullptr;        // behind the slabs; long rows only
         a.rows = rows; a.C = C;
         const LnShape s = ln_shape(C, dtype);
         if (dtype == DVAE_F32) ln_launch<float>(a, s, true, groups, S(st));

@@ -6,8 +6,11 @@
 //
 // Every statistic and sum is fp32 and taken from registers: the mean first, then the distances d from it.  sum(d) is what
 // rounding left of the mean and corrects both it and sum(d^2), so that a row whose mean is large against its spread (a
-// constant row at the extreme, where 1 / sqrt(eps) multiplies whatever is left) keeps its digits.  All orders are fixed:
-// results are bitwise reproducible, and a row's y and dx do not depend on the other rows of the call.
+// constant row at the extreme, where 1 / sqrt(eps) multiplies whatever is left) keeps its digits.  The backward pass starts from
+// the mean as it was stored, in one fp32 number, and takes what that lost from the sum of its own distances: with h = (x - mean) r
+// and c0 = mean(h), xh = h - c0 and mean(g xh) = mean(g h) - c0 mean(g), a third sum beside the two (at a mean of 1e6 spreads the
+// stored number alone puts xh off by 0.03).  All orders are fixed: results are bitwise reproducible, and a row's y and dx do not
+// depend on the other rows of the call.
 //
 // The bound is HBM: forward 2, backward 3 passes over the data.  A row lives in the registers of LPR lanes (a power of two,
 // as few as cover it with 16-byte vectors, so that narrow rows leave no lane idle) or of a whole workgroup; dgamma / dbeta
@@ -123,16 +126,22 @@ __device__ inline float wg_sum(float v, float* red) {
     return s;
 }
 
-// Two sums at once.
-template <int W>
-__device__ inline void wg_sum2(float& a, float& b, float (*red)[W]) {
-    a = row_sum<64>(a);
-    b = row_sum<64>(b);
-    if ((threadIdx.x & 63) == 0) { red[0][threadIdx.x >> 6] = a; red[1][threadIdx.x >> 6] = b; }
-    __syncthreads();
-    a = b = 0.f;
+// Several sums at once.
+template <int W, int K>
+__device__ inline void wg_sums(float (&v)[K], float (*red)[W]) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) { a += red[0][i]; b += red[1][i]; }
+    for (int k = 0; k < K; ++k) v[k] = row_sum<64>(v[k]);
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) red[k][threadIdx.x >> 6] = v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        v[k] = 0.f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[k] += red[k][i];
+    }
     __syncthreads();
 }
 
@@ -148,12 +157,25 @@ __device__ inline LnStat ln_stat(float sum_d, float sum_d2, float inv_c, float e
     return t;
 }
 
+// From the sums over a row of h, g and g h: the means the gradient takes away.
+struct LnMeans {
+    float c0, c1, c2;
+};
+__device__ inline LnMeans ln_means(float sum_h, float sum_g, float sum_gh, float inv_c) {
+    LnMeans t;
+    t.c0 = sum_h * inv_c;
+    t.c1 = sum_g * inv_c;
+    t.c2 = sum_gh * inv_c - t.c0 * t.c1;
+    return t;
+}
+
 struct LnArgs {
     const void *x, *dy;
     void* y;                       // y, or dx
     const float *gamma, *beta;
     float *mean, *invstd;          // [rows]: written forward (or NULL), read backward
     float* partial;                // backward: [gridDim.x][2][C], or NULL when neither dgamma nor dbeta is wanted
+    float* left;                   // backward, long rows: [rows], c0 for the columns' sums; or NULL
     long xs, ys, ds;               // row strides of x, y (dx), dy in elements
     long rows;
     int C;
@@ -262,33 +284,35 @@ __global__ __launch_bounds__(256) void ln_bwd_rows_kernel(LnArgs a) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) { vx[j] = nx[j]; vd[j] = nd[j]; }
         fetch(r + step);
-        float s1 = 0.f, s2 = 0.f;
+        float s0 = 0.f, s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int left = a.C - (j * LPR + lane) * N;
             const float m = ln_mean_of<TAIL, N>(mean, left);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float h = ln_only<TAIL>(((float)vx[j][i] - m) * inv, i, left), d = (float)vd[j][i], g = d * ga[j][i];
-                dg[j][i] += d * h;
-                db[j][i] += d;
+                const float h = ln_only<TAIL>(((float)vx[j][i] - m) * inv, i, left), g = (float)vd[j][i] * ga[j][i];
+                s0 += h;
                 s1 += g;
                 s2 += g * h;
             }
         }
-        // dx = inv (g - c1 - h c2)
-        const float c1 = row_sum<LPR>(s1) * inv_c, c2 = row_sum<LPR>(s2) * inv_c;
-        if (r < a.rows && dx) {
+        const LnMeans t = ln_means(row_sum<LPR>(s0), row_sum<LPR>(s1), row_sum<LPR>(s2), inv_c);
+        const bool put = r < a.rows && dx;
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int c = (j * LPR + lane) * N;
-                float o[N];
-                ln_forget(vx[j]);
-                ln_forget(vd[j]);
+        for (int j = 0; j < NV; ++j) {
+            const int c = (j * LPR + lane) * N;
+            float o[N];
+            ln_forget(vx[j]);
+            ln_forget(vd[j]);
 #pragma unroll
-                for (int i = 0; i < N; ++i) o[i] = inv * ((float)vd[j][i] * ga[j][i] - c1 - ((float)vx[j][i] - mean) * inv * c2);
-                ln_store<T, TAIL>(dx + r * a.ys + c, a.C - c, o);
+            for (int i = 0; i < N; ++i) {                // of columns that do not exist dy is zero, and nothing is stored
+                const float h = ((float)vx[j][i] - mean) * inv - t.c0, d = (float)vd[j][i];
+                dg[j][i] += d * h;
+                db[j][i] += d;
+                o[i] = inv * (d * ga[j][i] - t.c1 - h * t.c2);
             }
+            if (put) ln_store<T, TAIL>(dx + r * a.ys + c, a.C - c, o);
         }
     }
     if (!a.partial) return;
@@ -338,7 +362,7 @@ __global__ __launch_bounds__(W * 64) void ln_fwd_wide_kernel(LnArgs a) {
     fetch(blockIdx.x);
     for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
         float d[NV][N];
-        float s = 0.f, q = 0.f, e = 0.f;
+        float s = 0.f, eq[2] = {0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -355,12 +379,12 @@ __global__ __launch_bounds__(W * 64) void ln_fwd_wide_kernel(LnArgs a) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 d[j][i] = ln_only<TAIL>(d[j][i] - m, i, left);
-                e += d[j][i];
-                q += d[j][i] * d[j][i];
+                eq[0] += d[j][i];
+                eq[1] += d[j][i] * d[j][i];
             }
         }
-        wg_sum2<W>(e, q, red2);
-        const LnStat t = ln_stat(e, q, inv_c, a.eps);
+        wg_sums<W>(eq, red2);
+        const LnStat t = ln_stat(eq[0], eq[1], inv_c, a.eps);
         if (threadIdx.x == 0 && a.mean) { a.mean[r] = mean + t.off; a.invstd[r] = t.inv; }
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -376,7 +400,7 @@ template <typename T, int W, int NV, bool TAIL>
 __global__ __launch_bounds__(W * 64) void ln_bwd_wide_kernel(LnArgs a) {
     constexpr int N = LnVec<T>::N;
     constexpr bool AHEAD = NV * N <= 8;                  // 16 columns a thread leave no registers for the next row
-    __shared__ float red[2][W];
+    __shared__ float red[3][W];
     const T *x = (const T*)a.x, *dy = (const T*)a.dy;
     T* dx = (T*)a.y;
     float dg[NV][N], db[NV][N], ga[NV][N];
@@ -404,23 +428,21 @@ __global__ __launch_bounds__(W * 64) void ln_bwd_wide_kernel(LnArgs a) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) { vx[j] = nx[j]; vd[j] = nd[j]; }
         if (AHEAD) fetch(r + gridDim.x);
-        float s1 = 0.f, s2 = 0.f;
+        float s[3] = {0.f, 0.f, 0.f};                    // of h, g and g h
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int left = a.C - (j * W * 64 + (int)threadIdx.x) * N;
             const float m = ln_mean_of<TAIL, N>(mean, left);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float h = ln_only<TAIL>(((float)vx[j][i] - m) * inv, i, left), d = (float)vd[j][i], g = d * ga[j][i];
-                dg[j][i] += d * h;
-                db[j][i] += d;
-                s1 += g;
-                s2 += g * h;
+                const float h = ln_only<TAIL>(((float)vx[j][i] - m) * inv, i, left), g = (float)vd[j][i] * ga[j][i];
+                s[0] += h;
+                s[1] += g;
+                s[2] += g * h;
             }
         }
-        wg_sum2<W>(s1, s2, red);
-        const float c1 = s1 * inv_c, c2 = s2 * inv_c;
-        if (!dx) continue;
+        wg_sums<W>(s, red);
+        const LnMeans t = ln_means(s[0], s[1], s[2], inv_c);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int c = (j * W * 64 + (int)threadIdx.x) * N;
@@ -428,8 +450,13 @@ __global__ __launch_bounds__(W * 64) void ln_bwd_wide_kernel(LnArgs a) {
             ln_forget(vx[j]);
             ln_forget(vd[j]);
 #pragma unroll
-            for (int i = 0; i < N; ++i) o[i] = inv * ((float)vd[j][i] * ga[j][i] - c1 - ((float)vx[j][i] - mean) * inv * c2);
-            ln_store<T, TAIL>(dx + r * a.ys + c, a.C - c, o);
+            for (int i = 0; i < N; ++i) {
+                const float h = ((float)vx[j][i] - mean) * inv - t.c0, d = (float)vd[j][i];
+                dg[j][i] += d * h;
+                db[j][i] += d;
+                o[i] = inv * (d * ga[j][i] - t.c1 - h * t.c2);
+            }
+            if (dx) ln_store<T, TAIL>(dx + r * a.ys + c, a.C - c, o);
         }
     }
     if (!a.partial) return;
@@ -451,37 +478,41 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(LnArgs a) {
     for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T* x = (const T*)a.x + r * a.xs;
         T* y = (T*)a.y + r * a.ys;
-        float s = 0.f, q = 0.f, e = 0.f;
+        float s = 0.f, eq[2] = {0.f, 0.f};
         for (int c = threadIdx.x; c < a.C; c += 1024) s += (float)x[c];
         const float mean = wg_sum<16>(s, red) * inv_c;
-        for (int c = threadIdx.x; c < a.C; c += 1024) { const float d = (float)x[c] - mean; e += d; q += d * d; }
-        wg_sum2<16>(e, q, red2);
-        const LnStat t = ln_stat(e, q, inv_c, a.eps);
+        for (int c = threadIdx.x; c < a.C; c += 1024) { const float d = (float)x[c] - mean; eq[0] += d; eq[1] += d * d; }
+        wg_sums<16>(eq, red2);
+        const LnStat t = ln_stat(eq[0], eq[1], inv_c, a.eps);
         if (threadIdx.x == 0 && a.mean) { a.mean[r] = mean + t.off; a.invstd[r] = t.inv; }
         for (int c = threadIdx.x; c < a.C; c += 1024)
             y[c] = (T)(((float)x[c] - mean - t.off) * t.inv * (a.gamma ? a.gamma[c] : 1.f) + (a.beta ? a.beta[c] : 0.f));
     }
 }
 
-// dx of long rows; the columns' sums come from ln_cols_kernel
+// dx of long rows, and what the stored mean is off by, in spreads, for ln_cols_kernel, where the columns' sums come from
 template <typename T>
 __global__ __launch_bounds__(1024) void ln_bwd_long_kernel(LnArgs a) {
-    __shared__ float red[16];
+    __shared__ float red[3][16];
     const float inv_c = 1.f / (float)a.C;
     for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T *x = (const T*)a.x + r * a.xs, *dy = (const T*)a.dy + r * a.ds;
         T* dx = (T*)a.y + r * a.ys;
         const float mean = a.mean[r], inv = a.invstd[r];
-        float s1 = 0.f, s2 = 0.f;
+        float s[3] = {0.f, 0.f, 0.f};
         for (int c = threadIdx.x; c < a.C; c += 1024) {
-            const float g = (float)dy[c] * (a.gamma ? a.gamma[c] : 1.f);
-            s1 += g;
-            s2 += g * (((float)x[c] - mean) * inv);
+            const float g = (float)dy[c] * (a.gamma ? a.gamma[c] : 1.f), h = ((float)x[c] - mean) * inv;
+            s[0] += h;
+            s[1] += g;
+            s[2] += g * h;
         }
-        const float c1 = wg_sum<16>(s1, red) * inv_c, c2 = wg_sum<16>(s2, red) * inv_c;
+        wg_sums<16>(s, red);
+        const LnMeans t = ln_means(s[0], s[1], s[2], inv_c);
+        if (threadIdx.x == 0 && a.left) a.left[r] = t.c0;
+        if (!a.y) continue;
         for (int c = threadIdx.x; c < a.C; c += 1024) {
             const float g = (float)dy[c] * (a.gamma ? a.gamma[c] : 1.f);
-            dx[c] = (T)(inv * (g - c1 - ((float)x[c] - mean) * inv * c2));
+            dx[c] = (T)(inv * (g - t.c1 - (((float)x[c] - mean) * inv - t.c0) * t.c2));
         }
     }
 }
@@ -495,7 +526,7 @@ __global__ __launch_bounds__(256) void ln_cols_kernel(LnArgs a) {
     float dg = 0.f, db = 0.f;
     for (long r = blockIdx.y; r < a.rows; r += gridDim.y) {
         const float d = (float)dy[r * a.ds + c];
-        dg += d * (((float)x[r * a.xs + c] - a.mean[r]) * a.invstd[r]);
+        dg += d * (((float)x[r * a.xs + c] - a.mean[r]) * a.invstd[r] - a.left[r]);
         db += d;
     }
     float* out = a.partial + (long)blockIdx.y * 2 * a.C;
