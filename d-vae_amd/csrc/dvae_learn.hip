@@ -147,8 +147,9 @@ struct NsPlan {
 };
 
 // The largest singular value the iteration can reach from 1, and the largest |a + b s^2 + c s^4| it meets, by the polynomials'
-// own extrema.
-bool ns_coefficients_fit(double a, double b, double c, int steps) {
+// own extrema.  `rate`: the base-2 logarithm of the latter, rounded up and 0 at least.
+bool ns_coefficients_fit(double a, double b, double c, int steps, float& rate) {
+    double grows = 1.0;
     if (!isfinite(a) || !isfinite(b) || !isfinite(c)) return false;
     auto q = [&](double l) { return a + b * l + c * l * l; };
     double s = 1.0 + 1e-6;
@@ -170,6 +171,8 @@ bool ns_coefficients_fit(double a, double b, double c, int steps) {
         }
         for (int i = 0; i < n; ++i) most_x = fmax(most_x, sqrt(l[i]) * fabs(q(l[i])));
         if (!(most_q <= 7.001)) return false;                // a hair over, so that the bounds themselves pass
+        grows = fmax(grows, most_q);
+        rate = (float)(log2(grows) + 1e-6);
         s = most_x * (1.0 + 1e-4);
         if (!(s <= 2.001)) return false;
         if (s == 0.0) return true;
@@ -242,7 +245,7 @@ int ns_run_small(const char* what, const dvae_matrix* mats, int count, int scale
     static LdsOptIn opt[3];
     NsSmallArgs a{};
     a.eps = g.eps; a.a = g.a; a.b = g.b; a.c = g.c; a.mu = g.mu; a.nu = g.nu; a.lr = g.lr; a.decay = g.decay;
-    a.nesterov = g.nesterov; a.steps = steps;
+    a.nesterov = g.nesterov; a.steps = steps; a.rate = g.rate;
     std::vector<NsJob> many((size_t)(count > NS_SMALL_JOBS ? count : 0));
     NsJob* jobs = many.empty() ? a.jobs : many.data();
     int q = 1;
@@ -423,6 +426,7 @@ int ns_run(const char* what, const NsPlan& p, NsArgs g, int steps, hipStream_t s
     if (!p.matrices) return DVAE_OK;
     NS_LAUNCH(NS_SPLIT, ns_split_kernel<T, MUON>);
     for (int k = 0; k < steps; ++k) {
+        g.step = k;
         if (p.gram_ts == 32) {
             NS_LAUNCH_N(p.total[NS_GRAM], 2, 0, ns_direct_kernel<false, 8>);
             if (p.gram_pieces) NS_LAUNCH(NS_GRAM_TILES, ns_direct_sum_kernel);
@@ -460,11 +464,11 @@ int ns_run(const char* what, const NsPlan& p, NsArgs g, int steps, hipStream_t s
     return DVAE_OK;
 }
 
-int ns_iteration_check(const char* what, const double* coefficients, int steps, double eps) {
+int ns_iteration_check(const char* what, const double* coefficients, int steps, double eps, float& rate) {
     if (!coefficients) DVAE_FAIL(DVAE_EINVAL, "%s: null coefficients", what);
     if (steps < 1 || steps > 100) DVAE_FAIL(DVAE_EINVAL, "%s: %d steps (1 to 100)", what, steps);
     if (!(eps >= 0.0) || !isfinite(eps)) DVAE_FAIL(DVAE_EINVAL, "%s: eps %g", what, eps);
-    if (!ns_coefficients_fit(coefficients[0], coefficients[1], coefficients[2], steps))
+    if (!ns_coefficients_fit(coefficients[0], coefficients[1], coefficients[2], steps, rate))
         DVAE_FAIL(DVAE_EINVAL, "%s: coefficients (%g, %g, %g) leave the range this iteration is computed in: from singular "
                   "values up to 1 every step has to stay at 2 or below, with |a + b s^2 + c s^4| at 7 or below", what,
                   coefficients[0], coefficients[1], coefficients[2]);
@@ -562,11 +566,11 @@ int dvae_newton_schulz(const dvae_matrix* mats, int count, const double* coeffic
     try {
         int rc = ns_check("newton_schulz", mats, count, dtype, false);
         if (rc) return rc;
-        if ((rc = ns_iteration_check("newton_schulz", coefficients, steps, eps))) return rc;
+        NsArgs g{};
+        if ((rc = ns_iteration_check("newton_schulz", coefficients, steps, eps, g.rate))) return rc;
         for (int i = 0; i < count; ++i)
             if (mats[i].vector) DVAE_FAIL(DVAE_EINVAL, "newton_schulz: matrix %d is marked as a vector", i);
         if (count == 0) return DVAE_OK;
-        NsArgs g{};
         g.ws = (char*)workspace;
         g.a = (float)coefficients[0]; g.b = (float)coefficients[1]; g.c = (float)coefficients[2];
         g.eps = eps;
@@ -590,12 +594,12 @@ int dvae_muon_step(const dvae_matrix* mats, int count, double lr, double momentu
     try {
         int rc = ns_check("muon_step", mats, count, DVAE_F32, true);
         if (rc) return rc;
-        if ((rc = ns_iteration_check("muon_step", coefficients, steps, eps))) return rc;
+        NsArgs g{};
+        if ((rc = ns_iteration_check("muon_step", coefficients, steps, eps, g.rate))) return rc;
         if (scale_rule != DVAE_MUON_SPECTRAL && scale_rule != DVAE_MUON_RMS) DVAE_FAIL(DVAE_EINVAL, "muon_step: scale rule %d", scale_rule);
         if (!(momentum >= 0.0 && momentum < 1.0) || !(lr >= 0.0) || !(weight_decay >= 0.0) || !isfinite(lr * weight_decay))
             DVAE_FAIL(DVAE_EINVAL, "muon_step: lr %g, momentum %g, weight decay %g", lr, momentum, weight_decay);
         if (count == 0) return DVAE_OK;
-        NsArgs g{};
         g.ws = (char*)workspace;
         g.a = (float)coefficients[0]; g.b = (float)coefficients[1]; g.c = (float)coefficients[2];
         g.eps = eps;

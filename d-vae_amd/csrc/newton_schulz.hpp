@@ -7,9 +7,13 @@
 //
 // Number format.  The iteration multiplies small singular values by up to a^steps (485 for the usual coefficients), so
 // products of bf16 operands are off by 1 to 50 percent; fp32 operands would use the fp32 matrix rate, a sixteenth of
-// the 16-bit one.  Here an operand is the sum of two fp16 pieces, x = h + l (22 bits), and a product is three MFMAs,
-// hh + hl + lh, summed in fp32: the errors of an fp32 product at 3/16 of its time.  fp16's range is met by fixed scales: with
-// the coefficients' bounds checked on the host, |X| <= 2, |A| <= 4 and |B| <= 7, held as 2^14 X, 2^13 A and 2^13 B.
+// the 16-bit one.  Here an operand is the sum of two fp16 pieces, x = h + l / 2^11 (22 bits), and a product is three MFMAs,
+// hh + (hl + lh) / 2^11, summed in fp32: the errors of an fp32 product at 3/16 of its time.  fp16's range is met by scales: with
+// the coefficients' bounds checked on the host, |X| <= 2, |A| <= 4 and |B| <= 7, held as 2^14 X, 2^13 A and 2^13 B.  l's own
+// factor keeps it as far from fp16's lower end as h: without it elements below 6e-5 of the largest possible one would lose
+// digits (rows of 1e-6 of the others' size were off by 1.5e-4).  What is left is an absolute error of 2^-50 an element, against
+// matrices of norm up to 2: rows and columns of 1e-8 of the others' size are off by 1e-5, of 1e-10 by 1e-3.  A matrix that is small as
+// a whole, its norm far below eps, has a larger power of two than 2^14, see ns_shift.
 //
 // Layout.  An R x K operand is made of lines of 32 columns: a row's 32 h's, then its 32 l's, 128 bytes in eight chunks of 16.  Equal
 // chunks of the R rows follow each other, then the next chunk, then the next line: whatever a wave loads or stores, staged
@@ -33,7 +37,23 @@ using cgbytes = const DVAE_GLOBAL char*;
 template <typename T>
 __device__ inline DVAE_GLOBAL T* as_global(const void* p) { return (DVAE_GLOBAL T*)(uintptr_t)p; }
 
-constexpr float NS_SX = 16384.f, NS_SA = 8192.f, NS_SB = 8192.f;
+constexpr float NS_SX = 16384.f, NS_SA = 8192.f, NS_SB = 8192.f, NS_SL = 2048.f;
+
+// X_k is held as 2^(14 + shift) X_k: |X_0| is below 2^lead, lead the exponent of |X| / (|X| + eps), and a step multiplies every
+// singular value by at most 2^rate, rate >= 0 by the host's bound on |a + b s^2 + c s^4|.  Past 96 nothing of fp32's range is left
+// to be gained.
+__device__ inline int ns_shift(int lead, float rate, int step) {
+    const int v = -(lead + (int)ceilf(rate * (float)step));
+    return v < 0 ? 0 : v > 96 ? 96 : v;
+}
+__device__ inline int ns_lead(double norm, double eps) {
+    const double part = norm / (norm + eps);             // of a zero matrix without an eps, and of infinite ones, no number
+    int e = 0;
+    if (part > 0.0) (void)frexp(part, &e);
+    return e;
+}
+// 2^14 / (|X| + eps) from |X|^2
+__device__ inline double ns_inverse(double square, double eps) { return (double)NS_SX / (sqrt(square) + eps); }
 
 enum { NS_NORM, NS_SPLIT, NS_GRAM, NS_GRAM_TILES, NS_SQUARE, NS_APPLY, NS_PHASES };
 
@@ -60,6 +80,8 @@ struct NsArgs {
     int njobs, jp;
     int total;                // workgroups of this launch
     int turn;                 // which transposed copy is read
+    int step;
+    float rate;               // see ns_shift
     float a, b, c;
     double eps;
     NsJob one;                // the job, where there is only one: no table then
@@ -70,7 +92,7 @@ struct NsArgs {
 __host__ __device__ inline int ns_pad(int v) { return (v + 63) & ~63; }
 __host__ __device__ inline long ns_job_bytes(int m, int n) {
     const long p = ns_pad(m < n ? m : n), q = ns_pad(m < n ? n : m);
-    return 4 * (3 * p * q + 2 * p * p + p);              // A's diagonal last: p is a multiple of 64
+    return 4 * (3 * p * q + 2 * p * p + p + 64);         // A's diagonal and the matrix's lead last: p is a multiple of 64
 }
 
 // ---- the table of jobs -----------------------------------------------------------------------------------------------
@@ -121,6 +143,7 @@ struct NsPlanes {
     int P, Q;
     gbytes x, xt0, xt1, a, b;
     DVAE_GLOBAL float* diag;
+    DVAE_GLOBAL int* lead;
     __device__ NsPlanes(const NsArgs& g, const NsJob& j) {
         P = ns_pad(min(j.m, j.n));
         Q = ns_pad(max(j.m, j.n));
@@ -131,13 +154,15 @@ struct NsPlanes {
         a = x + 3 * pq;
         b = a + 4L * P * P;
         diag = (DVAE_GLOBAL float*)(b + 4L * P * P);
+        lead = (DVAE_GLOBAL int*)(diag + P);
     }
+    __device__ int shift(const NsArgs& g, int step) const { return ns_shift(*lead, g.rate, step); }
     __device__ gbytes xt(int which) const { return which ? xt1 : xt0; }
 };
 
 // A value that is about to be split is rounded to fp32 for good.  Left to itself the compiler converts a product to fp16 now
 // from its rounded value and now, fused, from its exact one; at a tie the h that is stored and the h that l is the rest of are
-// then two neighbours, and the pair is off by 2^-11.
+// then two neighbours, and the pair is off by 2^-11.  (What l is made from is exact: h's remainder times a power of two.)
 __device__ inline float ns_rounded(float v) {
     asm("" : "+v"(v));
     return v;
@@ -145,7 +170,7 @@ __device__ inline float ns_rounded(float v) {
 __device__ inline unsigned ns_split(float v) {           // low half: h, high half: l
     v = ns_rounded(v);
     const f16 h = (f16)v;
-    const f16 l = (f16)(v - (float)h);
+    const f16 l = (f16)((v - (float)h) * NS_SL);
     const f16x2 r = {h, l};
     return __builtin_bit_cast(unsigned, r);
 }
@@ -223,8 +248,11 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsArgs g) {
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
-    const double inv = (double)NS_SX / (sqrt((red[0] + red[1]) + (red[2] + red[3])) + g.eps);
+    s = (red[0] + red[1]) + (red[2] + red[3]);
     const NsPlanes w(g, j);
+    const int lead = ns_lead(sqrt(s), g.eps);
+    const double inv = ldexp(ns_inverse(s, g.eps), ns_shift(lead, g.rate, 0));
+    if (t == 0 && threadIdx.x == 0) *w.lead = lead;
     const bool tall = j.m > j.n;
     const int ncol = ns_pad(j.n) >> 6;
     const int r0 = t / ncol * 64, c0 = t % ncol * 64;
@@ -275,9 +303,10 @@ __device__ inline void ns_wave_sync() {
 }
 
 // ---- the products ----------------------------------------------------------------------------------------------------
-// C[i][k] = sum over c of L[i][c] R[k][c] for a TS x TS tile: four waves, a quarter tile each, 32x32x16 MFMAs.  Two LDS
-// stages of one line (32 columns) per row, one barrier a line: while one half of a line is multiplied, the fragments of the
-// other half are on their way from LDS, and the next two lines are on their way from memory in two sets of registers.
+// C[i][k] = sum over c of L[i][c] R[k][c] for a TS x TS tile: four waves, a quarter tile each, 32x32x16 MFMAs; hl + lh has sums of
+// its own.  Two LDS stages of one line (32 columns) per row, one barrier a line: while one half of a line is multiplied, the
+// fragments of the other half are on their way from LDS, and the next lines are on their way from memory, two in two sets of
+// registers, in tiles of 128, whose registers the sums take, one.
 // A line's eight 16-byte chunks are stored at chunk ^ (row / 2 & 7): of a fragment's rows any sixteen that are read at a time
 // meet the 64 banks once each.
 //
@@ -289,7 +318,8 @@ struct NsTile {
     static constexpr int PASS = TS / 32;                 // passes of 256 threads over a stage of one operand
     static constexpr int STAGES = 2 * 2 * TS * 128;      // bytes of a group
     static constexpr int BYTES = G * STAGES;
-    f32x16 acc[S][S];
+    static constexpr int SETS = S == 1 ? 2 : 1;          // lines on their way
+    f32x16 acc[S][S], low[S][S];
     int from = 0, to = S;                                // rows of subtiles that are this group's after join
 
     struct Lines { u32x4 l[PASS], r[PASS]; };
@@ -301,7 +331,7 @@ struct NsTile {
 #pragma unroll
             for (int k = 0; k < S; ++k)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) acc[i][k][e] = 0.f;
+                for (int e = 0; e < 16; ++e) acc[i][k][e] = low[i][k][e] = 0.f;
     }
 
     // MFMAs FROM to TO of the 3 S^2 of half a line
@@ -310,10 +340,12 @@ struct NsTile {
 #pragma unroll
         for (int m = FROM; m < TO; ++m) {
             const int w = m / (S * S), i = m / S % S, n = m % S;
-            acc[i][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w == 1 ? f.ll[i] : f.lh[i], w == 0 ? f.rl[n] : f.rh[n], acc[i][n], 0, 0, 0);
+            f32x16& c = w == 2 ? acc[i][n] : low[i][n];
+            c = __builtin_amdgcn_mfma_f32_32x32x16_f16(w == 1 ? f.ll[i] : f.lh[i], w == 0 ? f.rl[n] : f.rh[n], c, 0, 0, 0);
         }
     }
-    // `lines` is even; rows past lrows / rrows re-read the last one: their results are not stored
+    // `lines` is even.  Operands have multiples of 64 rows: where a tile of 128 has only 64, it reads those twice, and what comes of the
+    // second half is not stored.
     // SAME: both operands are the same rows, staged once.
     template <bool SAME = false>
     __device__ inline void run(cgbytes L, int lrows, int l0, cgbytes R, int rrows, int r0, int line0, int lines, char* smem) {
@@ -330,26 +362,19 @@ struct NsTile {
             line0 += group * lines;
             smem += group * STAGES;
         }
-        cgbytes lp[PASS], rp[PASS];
-#pragma unroll
-        for (int i = 0; i < PASS; ++i) {
-            lp[i] = L + (((long)line0 * 8 + chunk) * lrows + min(l0 + i * 32 + row, lrows - 1)) * 16;
-            rp[i] = R + (((long)line0 * 8 + chunk) * rrows + min(r0 + i * 32 + row, rrows - 1)) * 16;
-        }
-        Lines set[2];
+        cgbytes lp = L + (((long)line0 * 8 + chunk) * lrows + l0 + row) * 16, rp = R + (((long)line0 * 8 + chunk) * rrows + r0 + row) * 16;
+        const int lup = l0 + TS <= lrows ? 64 * 16 : 0, rup = r0 + TS <= rrows ? 64 * 16 : 0;
+        Lines set[SETS];
         int ahead = lines;
         auto fetch = [&](Lines& s) {                      // the next line; past the last one, that one again
 #pragma unroll
             for (int i = 0; i < PASS; ++i) {
-                s.l[i] = *(const DVAE_GLOBAL u32x4*)lp[i];
-                if (!SAME) s.r[i] = *(const DVAE_GLOBAL u32x4*)rp[i];
+                s.l[i] = *(const DVAE_GLOBAL u32x4*)(lp + (i >> 1) * lup + (i & 1) * 32 * 16);
+                if (!SAME) s.r[i] = *(const DVAE_GLOBAL u32x4*)(rp + (i >> 1) * rup + (i & 1) * 32 * 16);
             }
             const bool more = --ahead > 0;
-#pragma unroll
-            for (int i = 0; i < PASS; ++i) {
-                lp[i] += more ? lrows * 128L : 0L;
-                rp[i] += more ? rrows * 128L : 0L;
-            }
+            lp += more ? lrows * 128L : 0L;
+            rp += more ? rrows * 128L : 0L;
         };
         const int put = row * 128 + ((chunk ^ (row >> 1 & 7)) << 4);
         auto stage = [&](int at, const Lines& l) {
@@ -378,7 +403,7 @@ struct NsTile {
         };
         Frags f0, f1;
         fetch(set[0]);
-        fetch(set[1]);
+        if (SETS == 2) fetch(set[SETS - 1]);
         stage(0, set[0]);
         fetch(set[0]);
         __syncthreads();
@@ -388,15 +413,21 @@ struct NsTile {
             for (int d = 0; d < 2; ++d) {
                 read(f1, d, 1);
                 multiply<0, S * S>(f0);
-                stage(d ^ 1, set[d ^ 1]);
+                stage(d ^ 1, set[(d ^ 1) % SETS]);
                 multiply<S * S, 3 * S * S>(f0);
-                fetch(set[d ^ 1]);
+                fetch(set[(d ^ 1) % SETS]);
                 multiply<0, S * S>(f1);
                 __syncthreads();                          // this line's fragments are out, the next line is in
                 read(f0, d ^ 1, 0);
                 multiply<S * S, 3 * S * S>(f1);
             }
         }
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+#pragma unroll
+            for (int k = 0; k < S; ++k)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[i][k][e] += low[i][k][e] * (1.f / NS_SL);
     }
 
     // Adds the groups up: each keeps a row of subtiles.
@@ -526,8 +557,10 @@ __device__ inline float ns_polynomial(const Args& g, float square, float r, floa
 // element e of four pairs
 __device__ inline float ns_whole(u32x2 h, u32x2 l, int e) {
     const f16x2 hv = __builtin_bit_cast(f16x2, (unsigned)h[e >> 1]), lv = __builtin_bit_cast(f16x2, (unsigned)l[e >> 1]);
-    return (float)hv[e & 1] + (float)lv[e & 1];
+    return __builtin_fmaf((float)lv[e & 1], 1.f / NS_SL, (float)hv[e & 1]);
 }
+// What turns sums of products of X as it is held into A as it is held; 0 for an X so small that A is nothing beside a I.
+__device__ inline float ns_gram_scale(const NsArgs& g, const NsPlanes& w) { return ldexpf(NS_SA / (NS_SX * NS_SX), -2 * w.shift(g, g.step)); }
 // An element of A: R's, or, on the diagonal, none there and d's.
 __device__ inline float ns_off_diagonal(const NsPlanes& w, float v, int row, int col) {
     if (row != col) return v;
@@ -540,8 +573,9 @@ __device__ inline float ns_off_diagonal(const NsPlanes& w, float v, int row, int
 template <bool SQUARE>
 __device__ inline void ns_symmetric_value(const NsArgs& g, const NsPlanes& w, f32x16& v, int row, int col) {
     if (!SQUARE) {
+        const float scale = ns_gram_scale(g, w);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] *= NS_SA / (NS_SX * NS_SX);
+        for (int e = 0; e < 16; ++e) v[e] *= scale;
         if ((row ^ col) < 32) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) v[e] = ns_off_diagonal(w, v[e], row + 8 * (e >> 2) + (e & 3), col);
@@ -734,7 +768,7 @@ __global__ __launch_bounds__(64 * W) void ns_direct_kernel(NsArgs g) {
     for (int q = 0; q < 4; ++q) {
         f32x4 v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[0][4 * q + e] + acc[1][4 * q + e] + acc[2][4 * q + e];
+        for (int e = 0; e < 4; ++e) v[e] = acc[2][4 * q + e] + (acc[0][4 * q + e] + acc[1][4 * q + e]) * (1.f / NS_SL);
         red[wave][q][lane] = v;
     }
     __syncthreads();
@@ -757,9 +791,10 @@ __global__ __launch_bounds__(64 * W) void ns_direct_kernel(NsArgs g) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) f[e] = ns_polynomial(g, v[e], ns_whole(h, l, e), di[e], dk, row + e == col);
     } else {
+        const float scale = ns_gram_scale(g, w);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            f[e] = ns_off_diagonal(w, v[e] * (NS_SA / (NS_SX * NS_SX)), ti * 32 + 8 * wave + 4 * half + e, tk * 32 + (lane & 31));
+            f[e] = ns_off_diagonal(w, v[e] * scale, ti * 32 + 8 * wave + 4 * half + e, tk * 32 + (lane & 31));
     }
     ns_store_quarter(SQUARE ? w.b : w.a, rows, ti, tk, wave, f);
 }
@@ -785,9 +820,10 @@ __global__ __launch_bounds__(256) void ns_direct_sum_kernel(NsArgs g) {
             if (s + u < pieces) v += r[u];
     }
     float f[4];
+    const float scale = ns_gram_scale(g, w);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        f[e] = ns_off_diagonal(w, v[e] * (NS_SA / (NS_SX * NS_SX)), ti * 32 + 8 * wave + 4 * (lane >> 5) + e, tk * 32 + (lane & 31));
+        f[e] = ns_off_diagonal(w, v[e] * scale, ti * 32 + 8 * wave + 4 * (lane >> 5) + e, tk * 32 + (lane & 31));
     ns_store_quarter(w.a, w.P, ti, tk, wave, f);
 }
 
@@ -800,6 +836,7 @@ __global__ __launch_bounds__(256 * G, G == 1 ? 2 : 1) void ns_apply_kernel(NsArg
     const NsJob j = ns_job_of(g, ns_find(g, NS_APPLY, ns_swizzle(blockIdx.x, g.total), t));
     const NsPlanes w(g, j);
     const int ni = (w.P + TS - 1) / TS, ti = t % ni, tk = t / ni;
+    const float scale = ldexpf(1.f / NS_SB, w.shift(g, g.step + 1) - w.shift(g, g.step));
     NsTile<TS, G> c;
     c.zero();
     c.run(w.b, w.P, ti * TS, w.xt(g.turn), w.Q, tk * TS, 0, w.P / 32, smem);
@@ -813,7 +850,7 @@ __global__ __launch_bounds__(256 * G, G == 1 ? 2 : 1) void ns_apply_kernel(NsArg
             const int row = ti * TS + wr + i * 32, col = tk * TS + wc + k * 32;
             if (row >= w.P || col >= w.Q || i < c.from || i >= c.to) continue;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) c.acc[i][k][e] *= 1.f / NS_SB;
+            for (int e = 0; e < 16; ++e) c.acc[i][k][e] *= scale;
             ns_store(c.acc[i][k], patch, ns_line(w.x, w.P, row, col), w.P, ns_line(w.xt(g.turn ^ 1), w.Q, col, row), w.Q);
         }
 }
@@ -828,6 +865,7 @@ __global__ __launch_bounds__(256 * G, G == 1 ? 2 : 1) void ns_last_kernel(NsArgs
     const NsJob j = ns_job_of(g, ns_find(g, NS_APPLY, ns_swizzle(blockIdx.x, g.total), t));
     const NsPlanes w(g, j);
     const bool tall = j.m > j.n;
+    const float scale = ldexpf(1.f / (NS_SB * NS_SX), -w.shift(g, g.step));
     const int ni = (w.P + TS - 1) / TS, tp = t % ni, tq = t / ni;
     NsTile<TS, G> c;
     c.zero();
@@ -851,7 +889,7 @@ __global__ __launch_bounds__(256 * G, G == 1 ? 2 : 1) void ns_last_kernel(NsArgs
             const bool whole = ti * TS + NsTile<TS>::row_of(i, 15) < j.m;      // a lane's last row
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const float v = c.acc[i][k][e] * (1.f / (NS_SB * NS_SX));
+                const float v = c.acc[i][k][e] * scale;
                 p[e] = ns_rounded(MUON ? p[e] * g.decay - step * v : v);
             }
             if (whole) {

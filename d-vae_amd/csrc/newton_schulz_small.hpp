@@ -1,6 +1,6 @@
 // The whole iteration of a small matrix (p <= 64, q <= 768) in one workgroup and one launch: momentum, norm, every step, the
 // result or the parameter's update.  What bounds such matrices is not work (64 x 576: 0.3 GFLOP of MFMAs) but the chain of
-// dependent launches, four a step through the batched kernels, about 5 us each.  Measured: 64 x 576 47 us (7 a step), 64 x 27 20.5
+// dependent launches, four a step through the batched kernels, about 5 us each.  Measured: 64 x 576 48.5 us (7 a step), 64 x 27 21
 // (3 a step); what a step waits for is the chain of latencies below, and, with several blocks a wave, their conversions.
 //
 // Eight waves; wave w owns the 32-column blocks w, w + 8, .. of X (NB at most) and keeps them in registers for good, as
@@ -9,7 +9,8 @@
 //   Gram     every wave its blocks, 3 of the 4 subtiles of A (p x p), partial sums through LDS
 //   square   A in LDS as plane pairs, B = a I + b A + c A^2, two of its sixteen subtiles a wave, back to LDS
 //   apply    X^T <- X^T B, block by block: the one transposition (lanes to q) goes through a patch of LDS of the wave's own
-// Three barriers a step.  Numbers are held as in the batched kernels: two fp16 pieces, three MFMAs, fp32 sums.
+// Three barriers a step.  Numbers are held as in the batched kernels: two fp16 pieces, three MFMAs, fp32 sums,
+// those of hl and lh by themselves or first.
 #pragma once
 #include "newton_schulz.hpp"
 
@@ -26,6 +27,7 @@ struct NsSmallArgs {
     const NsJob* table;                                   // on the device, where there are more: then not NULL
     double eps;
     float a, b, c;
+    float rate;                                           // see ns_shift
     float mu, nu, lr, decay;
     int nesterov, steps;
 };
@@ -169,9 +171,12 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
     sq = 0.0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) sq += s.red[i];
-    // times 2^14 / (norm + eps), as a power of two and a factor near one: a float does not hold it for every norm
-    int shift;
-    const float factor = (float)frexp((double)NS_SX / (sqrt(sq) + g.eps), &shift);
+    // times 2^(14 + shift) / (norm + eps), as a power of two and a factor near one: a float does not hold it for every norm
+    int power;
+    const float factor = (float)frexp(ns_inverse(sq, g.eps), &power);
+    const int lead = ns_lead(sqrt(sq), g.eps);
+    int shift = ns_shift(lead, g.rate, 0);
+    power += shift;
 
     NsBlock blk[NB];
     // v times `by`, a power of two (so that the product is exact, see ns_rounded), in two pieces; element e of a subtile, e = 8 t + i, is element i of the fragment of half t
@@ -182,7 +187,7 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
             for (int e = 0; e < 8; ++e) {
                 const f16 h = (f16)(v[8 * t + e] * by);
                 b.h[i][t][e] = h;
-                b.l[i][t][e] = (f16)__builtin_fmaf(v[8 * t + e], by, -(float)h);
+                b.l[i][t][e] = (f16)(__builtin_fmaf(v[8 * t + e], by, -(float)h) * NS_SL);
             }
     };
 #pragma unroll
@@ -191,12 +196,14 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
         for (int i = 0; i < 2; ++i) {
             float v[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = ns_rounded(ldexpf(raw[k][i][e], shift) * factor);
+            for (int e = 0; e < 16; ++e) v[e] = ns_rounded(ldexpf(raw[k][i][e], power) * factor);
             hold(blk[k], i, v, 1.f);
         }
 
     const int used = min(8, (q + 31) / 32);               // waves that own a block
     for (int step = 0; step < g.steps; ++step) {
+        const int next = ns_shift(lead, g.rate, step + 1);
+        const float gram = ldexpf(NS_SA / (NS_SX * NS_SX), -2 * shift), back = ldexpf(1.f / NS_SB, next - shift);
         // ---- Gram ----
         if (wave < used) {
             const int lane = ns_lane();
@@ -205,18 +212,29 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
             for (int t = 0; t < 3; ++t)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[t][e] = 0.f;
+            // subtiles (0,0), (1,0), (1,1); first hl and lh of all blocks, a block past q holding zeros, then hh on top
 #pragma unroll
             for (int k = 0; k < NB; ++k) {
-                const NsBlock& b = blk[k];                // a block past q holds zeros
+                const NsBlock& b = blk[k];
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    // subtiles (0,0), (1,0), (1,1)
                     acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b.h[0][t], b.l[0][t], acc[0], 0, 0, 0);
                     acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b.h[1][t], b.l[0][t], acc[1], 0, 0, 0);
                     acc[2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b.h[1][t], b.l[1][t], acc[2], 0, 0, 0);
                     acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b.l[0][t], b.h[0][t], acc[0], 0, 0, 0);
                     acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b.l[1][t], b.h[0][t], acc[1], 0, 0, 0);
                     acc[2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b.l[1][t], b.h[1][t], acc[2], 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 3; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[t][e] *= 1.f / NS_SL;
+#pragma unroll
+            for (int k = 0; k < NB; ++k) {
+                const NsBlock& b = blk[k];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
                     acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b.h[0][t], b.h[0][t], acc[0], 0, 0, 0);
                     acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b.h[1][t], b.h[0][t], acc[1], 0, 0, 0);
                     acc[2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b.h[1][t], b.h[1][t], acc[2], 0, 0, 0);
@@ -253,13 +271,13 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
                 f16x2 h, l;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    float f = ns_rounded(v[t][i] * (NS_SA / (NS_SX * NS_SX)));
+                    float f = ns_rounded(v[t][i] * gram);
                     if (t != 1 && row + i == c) {
                         s.diag[c] = f;
                         f = 0.f;
                     }
                     h[i] = (f16)f;
-                    l[i] = (f16)(f - (float)h[i]);
+                    l[i] = (f16)((f - (float)h[i]) * NS_SL);
                 }
                 // the lane's two rows of column c are two columns of row c; the subtile below the diagonal is stored as it is, too
                 const int chunk = wave >> 1;
@@ -279,7 +297,7 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
         {
             const int lane = ns_lane(), r16 = lane & 15, quarter = lane >> 4;
             const int ti = wave >> 1;
-            f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+            f32x4 acc[2] = {}, low[2] = {};
 #pragma unroll
             for (int line = 0; line < 2; ++line) {
                 const f16x8 lh = *reinterpret_cast<const f16x8*>(s.a + ns_small_at(line, ti * 16 + r16, quarter));
@@ -292,9 +310,9 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
                     rl[n] = *reinterpret_cast<const f16x8*>(s.a + ns_small_at(line, row, 4 + quarter));
                 }
 #pragma unroll
-                for (int n = 0; n < 2; ++n) acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lh, rl[n], acc[n], 0, 0, 0);
+                for (int n = 0; n < 2; ++n) low[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lh, rl[n], low[n], 0, 0, 0);
 #pragma unroll
-                for (int n = 0; n < 2; ++n) acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ll, rh[n], acc[n], 0, 0, 0);
+                for (int n = 0; n < 2; ++n) low[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ll, rh[n], low[n], 0, 0, 0);
 #pragma unroll
                 for (int n = 0; n < 2; ++n) acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lh, rh[n], acc[n], 0, 0, 0);
             }
@@ -309,9 +327,10 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
                 f16x4 h, l;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float r = ns_rounded(ns_polynomial(g, acc[n][i], (float)vh[i] + (float)vl[i], dr[i], dc, r0 + i == c));
+                    const float r = ns_rounded(ns_polynomial(g, acc[n][i] + low[n][i] * (1.f / NS_SL), __builtin_fmaf((float)vl[i], 1.f / NS_SL, (float)vh[i]),
+                                                             dr[i], dc, r0 + i == c));
                     h[i] = (f16)r;
-                    l[i] = (f16)(r - (float)h[i]);
+                    l[i] = (f16)((r - (float)h[i]) * NS_SL);
                 }
                 *reinterpret_cast<f16x4*>(s.b + ah) = h;
                 *reinterpret_cast<f16x4*>(s.b + al) = l;
@@ -336,11 +355,11 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
                             *reinterpret_cast<f16x2*>(at + t * 16 * 256) = f16x2{blk[k].h[i][t][e], blk[k].l[i][t][e]};
                     }
                 ns_wave_sync();
-                f32x16 acc[2];
+                f32x16 acc[2], low[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
+                    for (int e = 0; e < 16; ++e) acc[i][e] = low[i][e] = 0.f;
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk) {
                     const int line = kk >> 1, t = kk & 1;
@@ -358,9 +377,9 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
                         rl[i] = *reinterpret_cast<const f16x8*>(s.b + ns_small_at(line, i * 32 + col, 4 + t * 2 + half));
                     }
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh, rl[i], acc[i], 0, 0, 0);
+                    for (int i = 0; i < 2; ++i) low[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh, rl[i], low[i], 0, 0, 0);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ll, rh[i], acc[i], 0, 0, 0);
+                    for (int i = 0; i < 2; ++i) low[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ll, rh[i], low[i], 0, 0, 0);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh, rh[i], acc[i], 0, 0, 0);
                 }
@@ -369,15 +388,16 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
                 for (int i = 0; i < 2; ++i) {
                     float v[16];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) v[e] = acc[i][e];
-                    hold(blk[k], i, v, 1.f / NS_SB);
+                    for (int e = 0; e < 16; ++e) v[e] = ns_rounded(acc[i][e] + low[i][e] * (1.f / NS_SL));
+                    hold(blk[k], i, v, back);
                 }
             }
         }
+        shift = next;
     }
 
     // ---- the result: back through the patch, so that lanes run along the caller's rows -------------------------------
-    const float step_len = MUON ? g.lr * j.scale : 0.f;
+    const float step_len = MUON ? g.lr * j.scale : 0.f, out_scale = ldexpf(1.f / NS_SX, -shift);
 #pragma unroll
     for (int k = 0; k < NB; ++k) {
         const int q0 = (wave + 8 * k) * 32;
@@ -387,7 +407,7 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsSmallArgs g) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
                     patch[(8 * (e >> 2) + 4 * half + (e & 3)) * PITCH + i * 32 + col] =
-                        ((float)blk[k].h[i][e >> 3][e & 7] + (float)blk[k].l[i][e >> 3][e & 7]) * (1.f / NS_SX);
+                        __builtin_fmaf((float)blk[k].l[i][e >> 3][e & 7], 1.f / NS_SL, (float)blk[k].h[i][e >> 3][e & 7]) * out_scale;
             ns_wave_sync();
 #pragma unroll
             for (int t = 0; t < 2; ++t) {

@@ -33,7 +33,8 @@ def newton_schulz(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
 
     ``x``: a float32 or bfloat16 device tensor of shape [..., m, n], or a list of them of one type (any shapes: the whole list
     is one batch of launches, 65536 matrices at most).  Returns the same, in x's type and layout.  The products have float32
-    accuracy for either type.  The result is not differentiable."""
+    accuracy for either type, as far as parts of a matrix go that are not below about 1e-7 of the rest (a row or column of
+    1e-8 of the others' size comes out to 1e-5 of itself).  The result is not differentiable."""
     many = isinstance(x, (list, tuple))
     xs = list(x) if many else [x]
     L.refuse_tangents("newton_schulz", *xs)

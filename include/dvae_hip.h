@@ -316,7 +316,10 @@ int dvae_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_
  * One call takes a list of matrices of any shapes (rows * cols < 2^31 each); the list is host memory and is read before the
  * call returns, whatever it points to is device memory.  Every matrix is divided by |X|_F + eps and goes `steps` times through
  *     A = X X^T,  X <- a X + (b A + c A^2) X        (coefficients = {a, b, c}; with rows > cols, as its transpose),
- * in products of fp32 accuracy whatever `dtype`, the type of x and out, is.  The coefficients have to keep the iteration
+ * in products of fp32 accuracy whatever `dtype`, the type of x and out, is: operands of 22 bits, fp32 sums.  Elements of X
+ * below 2^-28 (after the division) have an absolute error of 2^-50 instead: a row or column 1e-8 of the others' size comes out
+ * to 1e-5 of itself, one of 1e-10 to 1e-3, and what more steps make of it inherits that.  A matrix that is small as a whole,
+ * its norm far below eps, keeps its digits.  The coefficients have to keep the iteration
  * within singular values of 2 and |a + b s^2 + c s^4| within 7 (those in use do), else DVAE_EINVAL.  A matrix with a
  * non-finite element gives NaNs, a zero matrix zeros.  The workspace is 256-byte aligned. */
 typedef struct dvae_matrix {
