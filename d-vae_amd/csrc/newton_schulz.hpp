@@ -52,8 +52,8 @@ __device__ inline int ns_lead(double norm, double eps) {
     if (part > 0.0) (void)frexp(part, &e);
     return e;
 }
-// 2^14 / (|X| + eps) from |X|^2
-__device__ inline double ns_inverse(double square, double eps) { return (double)NS_SX / (sqrt(square) + eps); }
+// 2^14 / (|X| + eps) from |X|^2; a zero matrix stays one, whatever eps is
+__device__ inline double ns_inverse(double square, double eps) { return square == 0.0 ? 0.0 : (double)NS_SX / (sqrt(square) + eps); }
 
 enum { NS_NORM, NS_SPLIT, NS_GRAM, NS_GRAM_TILES, NS_SQUARE, NS_APPLY, NS_PHASES };
 

@@ -88,3 +88,45 @@ def test_muon_step_of_a_gradient_far_below_eps():
         want = -1e9 * s * ns(g.double())
         yard = -1e9 * s * ns(g).double()
         assert float((p.double() - want).norm()) <= 8 * float((yard - want).norm()) + 2.0 ** -19 * float(want.norm())
+
+
+SMALL, BATCHED = (40, 72), (100, 300)
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-320, 1e-7])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [SMALL, (72, 40), (60, 700), BATCHED, (300, 100)])
+def test_zero_matrix_comes_out_as_zeros(shape, dtype, eps):
+    """Whatever eps is: 0 / (0 + 0) is not taken.  The other matrix of the call is orthogonalised as ever."""
+    z, x = torch.zeros(shape, dtype=dtype, device="cuda"), noise(*shape, 5).to(dtype)
+    out = dvae_amd.newton_schulz([z, x], eps=eps)
+    assert not out[0].any() and torch.equal(out[1], dvae_amd.newton_schulz([x, x], eps=eps)[0])
+    if dtype == torch.float32:
+        p, m = torch.full(shape, 0.5, device="cuda"), torch.zeros(shape, device="cuda")
+        dvae_amd.muon_step([p], [z], [m], eps=eps, weight_decay=0.0)
+        assert bool((p == 0.5).all()) and not m.any()
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-7])
+@pytest.mark.parametrize("shape", [(1, 1), (5, 1), SMALL, (72, 40), (60, 700), BATCHED])
+def test_non_finite_matrices_stay_to_themselves(shape, eps):
+    """In the one-launch kernel as in the batched ones: NaNs all over, and nothing in the other matrices of the call."""
+    good = noise(*shape, 6)
+    nan, inf, both = good.clone(), good.clone(), good.clone()
+    nan[-1, 0], inf[0, -1] = float("nan"), float("-inf")
+    both[0, 0], both[-1, -1] = float("inf"), float("nan")
+    ref = dvae_amd.newton_schulz([good] * 5, eps=eps)[0]
+    out = dvae_amd.newton_schulz([nan, good, inf, good, both], eps=eps)
+    assert all(bool(out[i].isnan().all()) for i in (0, 2, 4))
+    assert torch.equal(out[1], ref) and torch.equal(out[3], ref)
+
+
+@pytest.mark.parametrize("shape", [BATCHED, (300, 100), (1100, 640)])
+def test_scale_of_the_input_in_the_batched_kernels(shape):
+    x = noise(*shape, 7) * 1e-3
+    ref = dvae_amd.newton_schulz(x)
+    for s in (1e25, 1e38 / float(x.abs().max()), 1.0):
+        y = dvae_amd.newton_schulz((x.double() * s).float())        # the factor itself leaves float32
+        # |x| + eps is 2e-7 of itself away from |x|, which 1e-7 of a step's slope at most makes of the result, beside the roundings
+        assert float((y - ref).norm()) <= 1e-4 * float(ref.norm())
+    held_everywhere(x * 1e-30, eps=1e-28)
