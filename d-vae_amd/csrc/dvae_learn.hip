@@ -338,7 +338,8 @@ int ns_plan(const char* what, const dvae_matrix* mats, int count, int scale_rule
     // The square has p / 32 lines and few tiles: straight from memory in tiles of 32 up to about two workgroups of those a SIMD
     // (beyond, they read more than the L2 gives), whole in tiles of 64 until those of 128 fill the chip.
     p.square_ts = tiles32 <= 1280 ? 32 : tiles[1][1] >= 512 ? 128 : 64;
-    // Two groups, see NsTile, where tiles of 128 are no more than the CUs (2048 x 2048: 68 -> 64 us).
+    // Two groups, see NsTile, where tiles of 128 are no more than the CUs.  Whole calls with one group and with two: 2048 x 2048 783
+    // and 770 us, 1984 x 2048 772 and 760, 1856 x 2048 648 and 636, 1000 x 4000 385 and 380, 832 x 4608 and 700 x 5000 the same.
     p.apply_groups = p.apply_ts == 128 && tiles[2][1] <= 256 ? 2 : 1;
     auto piece = [](bool cut, int kc, int all) {          // at most 64 of a tile; even
         if (!cut) return all;

@@ -314,6 +314,7 @@ __device__ inline void ns_wave_sync() {
 // no more tiles than CUs a CU has two waves a SIMD to cover each other's waits all the same.
 template <int TS, int G = 1>
 struct NsTile {
+    static_assert(G <= 2, "one group or two");
     static constexpr int S = TS / 64;                    // subtiles of a wave each way
     static constexpr int PASS = TS / 32;                 // passes of 256 threads over a stage of one operand
     static constexpr int STAGES = 2 * 2 * TS * 128;      // bytes of a group
@@ -351,16 +352,21 @@ struct NsTile {
     __device__ inline void run(cgbytes L, int lrows, int l0, cgbytes R, int rrows, int r0, int line0, int lines, char* smem) {
         const int tid = threadIdx.x & 255, row = tid & 31, chunk = tid >> 5, group = threadIdx.x >> 8;
         const int lane = tid & 63, wave = tid >> 6;
+        int idle = 0;                                     // lines that the other group has more
         if (G > 1) {
-            // where the lines do not make an even number for each, the first group takes all and the other keeps the barriers' count
-            const int active = lines % (2 * G) == 0 ? G : 1;
-            lines /= active;
-            if (group >= active) {
-                for (int k = 0; k <= lines; ++k) __syncthreads();
+            const int most = (lines / 2 + 1) & ~1;        // an even number for each
+            if (group) {
+                line0 += most;
+                lines -= most;
+                idle = most - lines;
+                smem += STAGES;
+            } else {
+                lines = most;
+            }
+            if (lines == 0) {
+                for (int k = 0; k <= idle; ++k) __syncthreads();
                 return;
             }
-            line0 += group * lines;
-            smem += group * STAGES;
         }
         cgbytes lp = L + (((long)line0 * 8 + chunk) * lrows + l0 + row) * 16, rp = R + (((long)line0 * 8 + chunk) * rrows + r0 + row) * 16;
         const int lup = l0 + TS <= lrows ? 64 * 16 : 0, rup = r0 + TS <= rrows ? 64 * 16 : 0;
@@ -422,6 +428,7 @@ struct NsTile {
                 multiply<S * S, 3 * S * S>(f1);
             }
         }
+        for (int k = 0; k < idle; ++k) __syncthreads();
 #pragma unroll
         for (int i = 0; i < S; ++i)
 #pragma unroll
