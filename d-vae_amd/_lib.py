@@ -149,6 +149,14 @@ def on_device(device):
     return torch.cuda.device(device)
 
 
+def capturing(device):
+    """Whether the current stream of ``device``, a tensor's, records a graph."""
+    if device.type != "cuda":
+        return False
+    with on_device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def refuse_tangents(what, *tensors):
     """Raises where a tensor carries a forward-mode tangent: a kernel sees only its value, and the result would silently have
     none.  Outside a dual level this is one comparison."""

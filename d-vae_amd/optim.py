@@ -140,7 +140,8 @@ def muon_step(params, grads, momenta, lr=0.02, momentum=0.95, nesterov=True, wei
 class FusedMuon(torch.optim.Optimizer):
     """Muon over ``muon_step``: a torch optimiser (schedulers, param groups, ``state_dict``) for float32 device parameters.
     Parameters without a gradient are skipped.  Groups may differ in any option; each group is one batch of launches.  A step
-    captured into a graph keeps the options it was captured with, and its replays change the weights without their models'
+    captured into a graph keeps the options it was captured with; the momenta have to exist before (one step outside the graph:
+    made inside, every replay would clear them, so that is refused).  Its replays change the weights without their models'
     knowledge: ``model._engine.invalidate()`` before such a model's next eager call, as after writes through ``param.data``."""
 
     _OPTIONS = ("lr", "momentum", "nesterov", "weight_decay", "steps", "coefficients", "eps", "scale")
@@ -168,6 +169,9 @@ class FusedMuon(torch.optim.Optimizer):
             for p in params:
                 state = self.state[p]
                 if "momentum_buffer" not in state:
+                    if L.capturing(p.device):
+                        raise RuntimeError("FusedMuon: the first step cannot be captured into a graph, whose replays would clear the "
+                                           "momenta that it makes: take one step before the capture")
                     state["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
                 momenta.append(state["momentum_buffer"])
             muon_step(params, [p.grad.contiguous() for p in params], momenta, **{k: group[k] for k in self._OPTIONS})
