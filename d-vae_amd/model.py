@@ -22,6 +22,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _lib as L
+from . import dist as D
 from .engine import DVAEConfig, DVAEEngine, bn_names, param_layout
 
 
@@ -62,7 +63,7 @@ class _PathFunction(torch.autograd.Function):
         eng = model._engine_for(x)
         b = x.shape[0]
         x0 = eng.input_from_nchw(x.detach().float())
-        e = eng.eps_from_nchw(eps) if eps is not None else eng.eps_philox(b, first=model._draws * b, stream_id=7)
+        e = eng.eps_from_nchw(eps) if eps is not None else eng.eps_philox(b, first=model._first_draw(b), stream_id=7)
         model._draws += 1
         train = model.training
         # mu / log_var are returned to the caller: they must be written (the fused inference head keeps them in registers)
@@ -261,6 +262,11 @@ class ResNetDVAE(nn.Module):
             names = self._path_names_cache = (cfg, ns)
         return names[1]
 
+    def _first_draw(self, b):
+        """First noise index of a call on ``b`` images: calls follow each other, and so do the ranks' parts of one call."""
+        rank, world = D.world_info()
+        return (self._draws * world + rank) * b
+
     def _cfg_for(self, S):
         c = self.engine_config()
         c.image_size = S
@@ -326,7 +332,7 @@ class ResNetDVAE(nn.Module):
         b, h = stem_out.shape[0], stem_out.shape[-1]
         a = eng.act("layer2.0.out" if self.stem_end_block == 7 else "layer2.1.out", h, 128)
         L.check(eng.lib.dvae_nchw_to_act(L.ptr(stem_out.contiguous().float()), L.ptr(a), b, 128, h, h, eng.dtype, L.stream()))
-        e = eng.eps_from_nchw(eps) if eps is not None else eng.eps_philox(b, first=self._draws * b, stream_id=7)
+        e = eng.eps_from_nchw(eps) if eps is not None else eng.eps_philox(b, first=self._first_draw(b), stream_id=7)
         self._draws += 1
         mulv, _, z = eng.latent(a, e, b, keep_eps=False)
         rec_pre = eng._decoder("decoder", z, b, self.training)

@@ -91,3 +91,22 @@ def test_generic_route_steps_the_global_batch(tmp_path, gate, epoch, cut):
         for r in range(2):
             for o, w in zip(got[r]["out"], out):
                 assert abs(o[k] - w[k]) <= 1e-5 * max(1.0, abs(w[k])), (k, o[k], w[k])
+
+
+def test_ranks_draw_noise_of_their_own(monkeypatch):
+    """The D-VAE's own noise, keyed by position: no index is drawn twice by the ranks of a call, or by two calls, and one
+    process draws what it always drew."""
+    import dvae_amd
+    model = dvae_amd.ResNet18DVAE(num_classes=10, stem_end_block=7, latent_dim=256)
+    seen = []
+    for world in (1, 3):
+        drawn = []
+        for call in range(4):
+            model._draws = call
+            for rank in range(world):
+                monkeypatch.setattr(D, "world_info", lambda rank=rank, world=world: (rank, world))
+                first = model._first_draw(5)
+                drawn += range(first, first + 5)
+        assert sorted(drawn) == list(range(4 * world * 5))
+        seen.append(drawn)
+    assert seen[0] == list(range(20))
