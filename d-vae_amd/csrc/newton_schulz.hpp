@@ -2,6 +2,7 @@
 //
 //   X_0 = X / (|X|_F + eps)     A = X X^T, B = a I + b A + c A^2, X <- B X      (`steps` times; p = min(m, n) rows)
 //
+// (K. Jordan and others, "Muon: an optimizer for hidden layers in neural networks", 2024, where the usual coefficients are from.)
 // (a I folded into B saves the third product an operand.)  A matrix with more rows than columns is iterated as its
 // transpose.  A list of matrices of any shapes runs as one batch: every phase is one launch over the tiles of all of them.
 //
@@ -553,7 +554,7 @@ __device__ inline void ns_store_symmetric(NsTile<TS>& c, char* smem, gbytes dst,
 // An element of B in row i, column k.  A is kept as its diagonal d, in fp32, and the rest R, in pieces: the matrix cores align the
 // products of a group to the largest and cut off what lies below its last bit, so that in A^2 the squares beside a dominant one of
 // the diagonal (X near orthogonal) lost some bits, always to one side.  In A^2 = R^2 + d_i R + R d_k + d^2 nothing is dominant:
-// 64 x 576 is off by 6.1e-7 instead of 1.7e-6 (fp32 products: 1.4e-6), for 0.5 to 4 % of the time.  `square` is R^2 (scaled), r the
+// 64 x 576 came from 1.7e-6 to 6.1e-7 by it (fp32 products: 1.4e-6), for 0.5 to 4 % of the time.  `square` is R^2 (scaled), r the
 // element of R.
 template <typename Args>
 __device__ inline float ns_polynomial(const Args& g, float square, float r, float di, float dk, bool diagonal) {

@@ -130,8 +130,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 
 
 class LayerNorm(nn.Module):
-    """torch.nn.LayerNorm over the last dimension (same parameter names) on ``layer_norm``.  The parameters stay float32,
-    whatever type the data has."""
+    """torch.nn.LayerNorm over the last dimension (same parameter names) on ``layer_norm``.  The parameters have to be
+    float32, whatever type the data has: after a ``.bfloat16()`` or ``.half()`` of the module its calls are refused."""
 
     def __init__(self, channels, eps=1e-5, affine=True):
         super().__init__()

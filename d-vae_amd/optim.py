@@ -138,8 +138,8 @@ def muon_step(params, grads, momenta, lr=0.02, momentum=0.95, nesterov=True, wei
 
 
 class FusedMuon(torch.optim.Optimizer):
-    """Muon over ``muon_step``: a torch optimiser (schedulers, param groups, ``state_dict``) for float32 device parameters.
-    Parameters without a gradient are skipped.  Groups may differ in any option; each group is one batch of launches.  A step
+    """Muon (K. Jordan and others, "Muon: an optimizer for hidden layers in neural networks", 2024) over ``muon_step``: a torch optimiser (schedulers, param groups, ``state_dict``) for contiguous float32 device
+    parameters.  Parameters without a gradient are skipped.  Groups may differ in any option; each group is one batch of launches.  A step
     captured into a graph keeps the options it was captured with; the momenta have to exist before (one step outside the graph:
     made inside, every replay would clear them, so that is refused).  Its replays change the weights without their models'
     knowledge: ``model._engine.invalidate()`` before such a model's next eager call, as after writes through ``param.data``."""

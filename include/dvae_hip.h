@@ -303,7 +303,7 @@ int dvae_clip_adam(float* p, const float* g, float* m, float* v, int64_t n, floa
  * one input row).  Pointers need the alignment of one element only.  gamma, beta and their gradients are fp32 [C], each
  * NULL if absent.  save_mean / save_invstd (fp32 [rows], both or neither) are what the backward pass reads; inference
  * passes NULL.  dx, dgamma and dbeta may each be NULL.  The workspace (16-byte aligned) is needed only for dgamma / dbeta.
- * C < 2^30; rows == 0 is allowed: the gradients of gamma and beta are then zero.  Bitwise reproducible; a row's results do
+ * Outputs overlap no input.  C < 2^30; rows == 0 is allowed: the gradients of gamma and beta are then zero.  Bitwise reproducible; a row's results do
  * not depend on the other rows. */
 size_t dvae_layer_norm_workspace_bytes(int64_t rows, int C, int dtype);
 int dvae_layer_norm_fwd(const void* x, int64_t x_stride, const float* gamma, const float* beta, void* y, int64_t y_stride,
@@ -321,7 +321,9 @@ int dvae_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_
  * to 1e-5 of itself, one of 1e-10 to 1e-3, and what more steps make of it inherits that.  A matrix that is small as a whole,
  * its norm far below eps, keeps its digits.  The coefficients have to keep the iteration
  * within singular values of 2 and |a + b s^2 + c s^4| within 7 (those in use do), else DVAE_EINVAL.  A matrix with a
- * non-finite element gives NaNs, a zero matrix zeros.  The workspace is 256-byte aligned. */
+ * non-finite element gives NaNs, a zero matrix zeros.  Results overlap neither each other nor a matrix of the list.  The workspace
+ * is 256-byte aligned; with p and q a matrix's sides padded to 64 it takes 4 (3 p q + 2 p^2) bytes for it beside tables and partial
+ * sums, next to nothing where all sides are at most 64 x 768. */
 typedef struct dvae_matrix {
     const void* x;            /* the matrix; dvae_muon_step: its gradient, fp32 */
     void* out;                /* the result; dvae_muon_step: the parameter, fp32, stepped in place */
