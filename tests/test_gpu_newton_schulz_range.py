@@ -34,7 +34,7 @@ def held_everywhere(x, steps=5, eps=1e-7):
         assert bool((off <= tol).all()), (dim, float((off / tol).max()), float((off / (size + 1e-300)).max()))
 
 
-SHAPES = [(40, 72), (64, 576), (700, 60), (100, 300), (600, 70), (512, 1500), (200, 9000), (1500, 2500)]
+SHAPES = [(40, 72), (50, 400), (64, 576), (700, 60), (100, 300), (600, 70), (512, 1500), (200, 9000), (1500, 2500)]
 
 
 @pytest.mark.parametrize("m,n", SHAPES)
